@@ -140,6 +140,14 @@ class PagedPrefillArgs(C.Structure):
                 ("out_dtype", C.c_uint32), ("scale", C.c_float)]
 
 
+class Q8Cache(C.Structure):
+    _fields_ = [("k_scales", C.c_void_p), ("v_scales", C.c_void_p), ("cache_dtype", C.c_uint32)]
+
+
+class AttentionWindow(C.Structure):
+    _fields_ = [("window", C.c_uint32), ("sinks", C.c_uint32)]
+
+
 class KernelTiming(C.Structure):
     _fields_ = [("name", C.c_char * 64), ("gpu_time_ms", C.c_double), ("dispatches", C.c_uint64)]
 
@@ -187,6 +195,16 @@ _sig("granite_cuda_rope_multihead", C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
 _sig("granite_cuda_rope_paged_kv_cache_append", C.c_int, C.c_void_p, C.POINTER(RopeAppendArgs))
 _sig("granite_cuda_tree_commit", C.c_int, C.c_void_p, C.POINTER(TreeCommitArgs))
 _sig("granite_cuda_paged_prefill_attention", C.c_int, C.c_void_p, C.POINTER(PagedPrefillArgs))
+_sig("granite_cuda_rope_paged_kv_cache_append_q8", C.c_int, C.c_void_p, C.POINTER(RopeAppendArgs), C.POINTER(Q8Cache))
+_sig("granite_cuda_batched_paged_attention_decode_q8", C.c_int, C.c_void_p, C.POINTER(PagedDecodeArgs), C.POINTER(Q8Cache),
+     C.POINTER(AttentionWindow))
+_sig("granite_cuda_paged_prefill_attention_q8", C.c_int, C.c_void_p, C.POINTER(PagedPrefillArgs), C.POINTER(Q8Cache),
+     C.POINTER(AttentionWindow))
+_sig("granite_cuda_batched_paged_attention_decode_window", C.c_int, C.c_void_p, C.POINTER(PagedDecodeArgs),
+     C.POINTER(AttentionWindow))
+_sig("granite_cuda_multihead_attention_window", C.c_int, C.c_void_p, C.POINTER(AttentionArgs), C.POINTER(AttentionWindow))
+_sig("granite_cuda_paged_prefill_attention_window", C.c_int, C.c_void_p, C.POINTER(PagedPrefillArgs),
+     C.POINTER(AttentionWindow))
 _sig("granite_cuda_selftest_bounded_wait", C.c_int, C.c_void_p, C.c_uint64, C.c_void_p)
 _sig("granite_cuda_push_rows", C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p), C.c_uint32,
      C.c_uint64, C.c_uint64)
@@ -390,6 +408,63 @@ class CudaCompute:
                              num_kv_heads, seq_q, start_pos, head_dim, block_size, max_blocks_per_seq, num_blocks,
                              q_dtype, out_dtype, scale)
         check(lib.granite_cuda_paged_prefill_attention(self._h, C.byref(a)))
+
+    # ---- 8-bit paged cache (cache_dtype 0: int8, 1: fp8 e4m3) and sliding windows; window 0 on the 8-bit calls: none
+    def rope_paged_kv_cache_append_q8(self, q, k, v, cos_table, sin_table, K_cache, V_cache, k_scales, v_scales,
+                                      block_tables, positions, batch_size, new_len, num_heads, num_kv_heads, head_dim,
+                                      block_size, max_blocks_per_seq, num_blocks, table_len, cache_dtype,
+                                      start_pos=0) -> None:
+        a = RopeAppendArgs(_ptr(q), _ptr(k), _ptr(v), _ptr(cos_table), _ptr(sin_table), _ptr(K_cache),
+                           _ptr(V_cache), _ptr(block_tables), _ptr(positions), batch_size, new_len, num_heads,
+                           num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks, table_len, start_pos)
+        x = Q8Cache(_ptr(k_scales), _ptr(v_scales), cache_dtype)
+        check(lib.granite_cuda_rope_paged_kv_cache_append_q8(self._h, C.byref(a), C.byref(x)))
+
+    def batched_paged_attention_decode_q8(self, Q, K_cache, V_cache, k_scales, v_scales, block_tables, seq_lens, output,
+                                          batch_size, num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq,
+                                          scale, *, num_blocks, cache_dtype, seq_len=0, window=0, sinks=0) -> None:
+        a = PagedDecodeArgs(_ptr(Q), _ptr(K_cache), _ptr(V_cache), _ptr(block_tables), _ptr(seq_lens),
+                            _ptr(output), batch_size, num_heads, num_kv_heads, head_dim, block_size,
+                            max_blocks_per_seq, num_blocks, seq_len, scale)
+        x = Q8Cache(_ptr(k_scales), _ptr(v_scales), cache_dtype)
+        w = C.byref(AttentionWindow(window, sinks)) if window else None
+        check(lib.granite_cuda_batched_paged_attention_decode_q8(self._h, C.byref(a), C.byref(x), w))
+
+    def paged_prefill_attention_q8(self, Q, K_cache, V_cache, k_scales, v_scales, block_table, output, num_heads,
+                                   num_kv_heads, seq_q, start_pos, head_dim, block_size, max_blocks_per_seq, num_blocks,
+                                   scale, cache_dtype, q_dtype=0, out_dtype=0, window=0, sinks=0) -> None:
+        a = PagedPrefillArgs(_ptr(Q), _ptr(K_cache), _ptr(V_cache), _ptr(block_table), _ptr(output), num_heads,
+                             num_kv_heads, seq_q, start_pos, head_dim, block_size, max_blocks_per_seq, num_blocks,
+                             q_dtype, out_dtype, scale)
+        x = Q8Cache(_ptr(k_scales), _ptr(v_scales), cache_dtype)
+        w = C.byref(AttentionWindow(window, sinks)) if window else None
+        check(lib.granite_cuda_paged_prefill_attention_q8(self._h, C.byref(a), C.byref(x), w))
+
+    def batched_paged_attention_decode_window(self, Q, K_cache, V_cache, block_tables, seq_lens, output, batch_size,
+                                              num_heads, num_kv_heads, head_dim, block_size, max_blocks_per_seq, scale,
+                                              window, sinks=0, *, num_blocks, seq_len=0) -> None:
+        a = PagedDecodeArgs(_ptr(Q), _ptr(K_cache), _ptr(V_cache), _ptr(block_tables), _ptr(seq_lens),
+                            _ptr(output), batch_size, num_heads, num_kv_heads, head_dim, block_size,
+                            max_blocks_per_seq, num_blocks, seq_len, scale)
+        w = AttentionWindow(window, sinks)
+        check(lib.granite_cuda_batched_paged_attention_decode_window(self._h, C.byref(a), C.byref(w)))
+
+    def multihead_attention_window(self, Q, K, V, output, num_heads, num_kv_heads, seq_q, seq_kv, head_dim, scale,
+                                   window, sinks=0, max_seq=0, *, q_dtype=0, out_dtype=0, start_pos=0,
+                                   batch_size=1) -> None:
+        a = AttentionArgs(_ptr(Q), _ptr(K), _ptr(V), _ptr(output), num_heads, num_kv_heads, seq_q,
+                          seq_kv, head_dim, max_seq, q_dtype, out_dtype, scale, start_pos, batch_size)
+        w = AttentionWindow(window, sinks)
+        check(lib.granite_cuda_multihead_attention_window(self._h, C.byref(a), C.byref(w)))
+
+    def paged_prefill_attention_window(self, Q, K_cache, V_cache, block_table, output, num_heads, num_kv_heads, seq_q,
+                                       start_pos, head_dim, block_size, max_blocks_per_seq, num_blocks, scale, window,
+                                       sinks=0, q_dtype=0, out_dtype=0) -> None:
+        a = PagedPrefillArgs(_ptr(Q), _ptr(K_cache), _ptr(V_cache), _ptr(block_table), _ptr(output), num_heads,
+                             num_kv_heads, seq_q, start_pos, head_dim, block_size, max_blocks_per_seq, num_blocks,
+                             q_dtype, out_dtype, scale)
+        w = AttentionWindow(window, sinks)
+        check(lib.granite_cuda_paged_prefill_attention_window(self._h, C.byref(a), C.byref(w)))
 
     def selftest_bounded_wait(self, limit_cycles: int, released_early) -> None:
         check(lib.granite_cuda_selftest_bounded_wait(self._h, limit_cycles, C.c_void_p(_ptr(released_early))))

@@ -258,6 +258,7 @@ int granite_cuda_sync(granite_cuda_compute_t* c) {
     if (st & kStatusBadTable) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "a block-table entry was outside the pool");
     if (st & kStatusBadSeqLen) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "a sequence length was negative or exceeded its block table");
     if (st & kStatusBadParent) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "a tree parent index was out of range");
+    if (st & kStatusNonFinite) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "a K or V value for the 8-bit cache was NaN or infinite (stored as 0)");
     if (st & kStatusLayout) return fail(GRANITE_CUDA_INTERNAL_ERROR, "a kernel's shared-memory layout did not fit its window");
     return fail(GRANITE_CUDA_EXECUTION_FAILED, "device status " + std::to_string(st));
 }
@@ -380,26 +381,33 @@ int granite_cuda_batched_paged_attention_decode_gather_heads(granite_cuda_comput
     return launch_paged_decode(c, *args, false, 0, &g);
 }
 
+// One query row over a contiguous cache is a decode; the arguments it has there.
+static int contiguous_decode_args(const GraniteCudaAttentionArgs& a, GraniteCudaPagedDecodeArgs* d, uint32_t* max_seq) {
+    *max_seq = a.max_seq ? a.max_seq : a.seq_kv;
+    if (a.q_dtype != 0 || a.out_dtype != 0)
+        return fail(GRANITE_CUDA_INVALID_ARGUMENT, "decode takes fp32 Q and writes fp32");
+    if (a.seq_kv > *max_seq) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "seq_kv exceeds max_seq");
+    d->q = static_cast<const float*>(a.q);
+    d->k_cache = a.k;
+    d->v_cache = a.v;
+    d->output = static_cast<float*>(a.output);
+    d->batch_size = a.batch_size ? a.batch_size : 1;
+    d->num_heads = a.num_heads;
+    d->num_kv_heads = a.num_kv_heads;
+    d->head_dim = a.head_dim;
+    d->block_size = 16;
+    d->seq_len = a.seq_kv;
+    d->scale = a.scale;
+    return GRANITE_CUDA_SUCCESS;
+}
+
 int granite_cuda_multihead_attention(granite_cuda_compute_t* c, const GraniteCudaAttentionArgs* a) {
     if (!c || !a) return fail(GRANITE_CUDA_NULL_POINTER, "multihead_attention: null argument");
     GB_CUDA_TRY(cudaSetDevice(c->device));
-    const uint32_t max_seq = a->max_seq ? a->max_seq : a->seq_kv;
     if (a->seq_q == 1) {
-        if (a->q_dtype != 0 || a->out_dtype != 0)
-            return fail(GRANITE_CUDA_INVALID_ARGUMENT, "decode takes fp32 Q and writes fp32");
-        if (a->seq_kv > max_seq) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "seq_kv exceeds max_seq");
         GraniteCudaPagedDecodeArgs d{};
-        d.q = static_cast<const float*>(a->q);
-        d.k_cache = a->k;
-        d.v_cache = a->v;
-        d.output = static_cast<float*>(a->output);
-        d.batch_size = a->batch_size ? a->batch_size : 1;
-        d.num_heads = a->num_heads;
-        d.num_kv_heads = a->num_kv_heads;
-        d.head_dim = a->head_dim;
-        d.block_size = 16;
-        d.seq_len = a->seq_kv;
-        d.scale = a->scale;
+        uint32_t max_seq = 0;
+        if (int rc = contiguous_decode_args(*a, &d, &max_seq)) return rc;
         return launch_paged_decode(c, d, true, max_seq);
     }
     return launch_prefill(c, *a);
@@ -483,6 +491,99 @@ int granite_cuda_paged_prefill_attention(granite_cuda_compute_t* c, const Granit
     if (!c || !args) return fail(GRANITE_CUDA_NULL_POINTER, "paged_prefill_attention: null argument");
     GB_CUDA_TRY(cudaSetDevice(c->device));
     return launch_paged_prefill(c, *args);
+}
+
+// The calls below check their own arguments before the compute object, so that a refusal needs no device.
+static int view_of(const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window, bool window_required,
+                   const void* k_pool, const void* v_pool, const char* what, CacheView* out) {
+    if (cache) {
+        if (!cache->k_scales || !cache->v_scales) return fail(GRANITE_CUDA_NULL_POINTER, std::string(what) + ": null scales");
+        if (cache->cache_dtype > 1)
+            return fail(GRANITE_CUDA_INVALID_ARGUMENT, std::string(what) + ": cache_dtype must be 0 (int8) or 1 (e4m3)");
+        if ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15)
+            return fail(GRANITE_CUDA_INVALID_ARGUMENT, std::string(what) + ": the pools must be 16-byte aligned");
+        out->elem = 1 + (int)cache->cache_dtype;
+        out->k_scales = cache->k_scales;
+        out->v_scales = cache->v_scales;
+    }
+    if (window_required && !window) return fail(GRANITE_CUDA_NULL_POINTER, std::string(what) + ": window is null");
+    if (window) {
+        if (window->window == 0) return fail(GRANITE_CUDA_INVALID_ARGUMENT, std::string(what) + ": window must be at least 1");
+        out->window = window->window;
+        out->sinks = window->sinks;
+    }
+    return GRANITE_CUDA_SUCCESS;
+}
+
+int granite_cuda_rope_paged_kv_cache_append_q8(granite_cuda_compute_t* c, const GraniteCudaRopeAppendArgs* args,
+                                               const GraniteCudaQ8Cache* cache) {
+    if (!args || !cache) return fail(GRANITE_CUDA_NULL_POINTER, "rope_paged_kv_cache_append_q8: null argument");
+    if (int rc = check_q8_append(*args, *cache)) return rc;
+    if (!c) return fail(GRANITE_CUDA_NULL_POINTER, "rope_paged_kv_cache_append_q8: compute object is null");
+    GB_CUDA_TRY(cudaSetDevice(c->device));
+    return launch_q8_append(c, *args, *cache);
+}
+
+int granite_cuda_batched_paged_attention_decode_q8(granite_cuda_compute_t* c, const GraniteCudaPagedDecodeArgs* args,
+                                                   const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window) {
+    if (!args || !cache) return fail(GRANITE_CUDA_NULL_POINTER, "paged decode q8: null argument");
+    CacheView view;
+    if (int rc = view_of(cache, window, false, args->k_cache, args->v_cache, "paged decode q8", &view)) return rc;
+    if (int rc = check_decode_view(*args, false, 0)) return rc;
+    if (!c) return fail(GRANITE_CUDA_NULL_POINTER, "paged decode q8: compute object is null");
+    GB_CUDA_TRY(cudaSetDevice(c->device));
+    return launch_decode_view(c, *args, false, 0, view);
+}
+
+int granite_cuda_paged_prefill_attention_q8(granite_cuda_compute_t* c, const GraniteCudaPagedPrefillArgs* args,
+                                            const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window) {
+    if (!args || !cache) return fail(GRANITE_CUDA_NULL_POINTER, "paged_prefill_attention_q8: null argument");
+    CacheView view;
+    if (int rc = view_of(cache, window, false, args->k_cache, args->v_cache, "paged_prefill_attention_q8", &view)) return rc;
+    if (int rc = check_paged_prefill_view(*args)) return rc;
+    if (!c) return fail(GRANITE_CUDA_NULL_POINTER, "paged_prefill_attention_q8: compute object is null");
+    GB_CUDA_TRY(cudaSetDevice(c->device));
+    return launch_paged_prefill_view(c, *args, view);
+}
+
+int granite_cuda_batched_paged_attention_decode_window(granite_cuda_compute_t* c, const GraniteCudaPagedDecodeArgs* args,
+                                                       const GraniteCudaAttentionWindow* window) {
+    if (!args) return fail(GRANITE_CUDA_NULL_POINTER, "paged decode window: null argument");
+    CacheView view;
+    if (int rc = view_of(nullptr, window, true, nullptr, nullptr, "paged decode window", &view)) return rc;
+    if (int rc = check_decode_view(*args, false, 0)) return rc;
+    if (!c) return fail(GRANITE_CUDA_NULL_POINTER, "paged decode window: compute object is null");
+    GB_CUDA_TRY(cudaSetDevice(c->device));
+    return launch_decode_view(c, *args, false, 0, view);
+}
+
+int granite_cuda_multihead_attention_window(granite_cuda_compute_t* c, const GraniteCudaAttentionArgs* a,
+                                            const GraniteCudaAttentionWindow* window) {
+    if (!a) return fail(GRANITE_CUDA_NULL_POINTER, "multihead_attention_window: null argument");
+    CacheView view;
+    if (int rc = view_of(nullptr, window, true, nullptr, nullptr, "multihead_attention_window", &view)) return rc;
+    GraniteCudaPagedDecodeArgs d{};
+    uint32_t max_seq = 0;
+    if (a->seq_q == 1) {
+        if (int rc = contiguous_decode_args(*a, &d, &max_seq)) return rc;
+        if (int rc = check_decode_view(d, true, max_seq)) return rc;
+    } else if (int rc = check_prefill_view(*a)) {
+        return rc;
+    }
+    if (!c) return fail(GRANITE_CUDA_NULL_POINTER, "multihead_attention_window: compute object is null");
+    GB_CUDA_TRY(cudaSetDevice(c->device));
+    return a->seq_q == 1 ? launch_decode_view(c, d, true, max_seq, view) : launch_prefill_view(c, *a, view);
+}
+
+int granite_cuda_paged_prefill_attention_window(granite_cuda_compute_t* c, const GraniteCudaPagedPrefillArgs* args,
+                                                const GraniteCudaAttentionWindow* window) {
+    if (!args) return fail(GRANITE_CUDA_NULL_POINTER, "paged_prefill_attention_window: null argument");
+    CacheView view;
+    if (int rc = view_of(nullptr, window, true, nullptr, nullptr, "paged_prefill_attention_window", &view)) return rc;
+    if (int rc = check_paged_prefill_view(*args)) return rc;
+    if (!c) return fail(GRANITE_CUDA_NULL_POINTER, "paged_prefill_attention_window: compute object is null");
+    GB_CUDA_TRY(cudaSetDevice(c->device));
+    return launch_paged_prefill_view(c, *args, view);
 }
 
 int granite_cuda_selftest_bounded_wait(granite_cuda_compute_t* c, uint64_t limit_cycles, int32_t* released_early) {

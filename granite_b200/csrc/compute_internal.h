@@ -22,6 +22,7 @@ enum : int {
     kStatusBadSeqLen = 4,    // a sequence length outside [0, max_blocks*block_size]
     kStatusBadParent = 8,    // a tree parent index outside [-1, num_nodes)
     kStatusLayout = 16,      // a kernel found its shared-memory window smaller than its layout
+    kStatusNonFinite = 32,   // a K or V value for the 8-bit cache was NaN or infinite
 };
 
 // The status word and, 256 bytes behind it, the arrival counters of the one-launch decode (one per (sequence,
@@ -155,10 +156,29 @@ int launch_rope_multihead(granite_cuda_compute* c, float* q, float* k, uint32_t 
 int launch_rope_paged_append(granite_cuda_compute* c, const GraniteCudaRopeAppendArgs& a);
 int launch_tree_commit(granite_cuda_compute* c, const GraniteCudaTreeCommitArgs& a);
 int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a);
+// What distinguishes an 8-bit or windowed attention call from the plain one: the cache's element type and scales (elem as
+// in q8.cuh: 0 fp16, 1 int8, 2 e4m3) and the window (0: none).
+struct CacheView {
+    int elem = 0;
+    const float* k_scales = nullptr;
+    const float* v_scales = nullptr;
+    uint32_t window = 0, sinks = 0;
+};
 // plain fp32 kernel for head dims, page sizes and head counts outside the tuned kernels' shapes
-int launch_generic_decode(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq);
-int launch_generic_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a);
-int launch_generic_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a);
+int launch_generic_decode(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq,
+                          const CacheView& view = CacheView{});
+int launch_generic_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, const CacheView& view = CacheView{});
+int launch_generic_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a, const CacheView& view = CacheView{});
+// the calls that see the cache through a view, and their argument checks, which need no device (the entry points make
+// them before anything else)
+int check_decode_view(const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq);
+int check_prefill_view(const GraniteCudaAttentionArgs& a);
+int check_paged_prefill_view(const GraniteCudaPagedPrefillArgs& a);
+int launch_decode_view(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq, const CacheView& view);
+int launch_prefill_view(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, const CacheView& view);
+int launch_paged_prefill_view(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a, const CacheView& view);
+int check_q8_append(const GraniteCudaRopeAppendArgs& a, const GraniteCudaQ8Cache& x);
+int launch_q8_append(granite_cuda_compute* c, const GraniteCudaRopeAppendArgs& a, const GraniteCudaQ8Cache& x);
 int launch_generic_tree(granite_cuda_compute* c, const GraniteCudaTreeAttentionArgs& a);
 int launch_bounded_wait_selftest(granite_cuda_compute* c, uint64_t limit_cycles, int* released_early_dev);
 int launch_push_rows(granite_cuda_compute* c, cudaStream_t stream, const void* src, void* const* dst_ptrs, uint32_t n_dst,

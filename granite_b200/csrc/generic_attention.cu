@@ -9,8 +9,13 @@
 // Arithmetic as in src/llm/transformer.mm:1779-1840 (scores = (q . k) * scale, causal rule
 // k_pos > start_pos + q_pos) and :2044-2126 (tree: whole prefix, then the node itself and its
 // ancestors, :823-840).
+//
+// The 8-bit caches and the sliding window go through the same kernel, built separately (kElem, kWindow): codes
+// become fp32 as they are read, a page's K scale multiplies the score and its V scale the weight; a window leaves the keys
+// [0, sinks) and [lo, pos], which the loop walks as one list, so hidden pages are neither read nor looked up.
 #include "compute_internal.h"
 #include "ptx.cuh"
+#include "q8.cuh"
 
 namespace gb200 {
 
@@ -22,8 +27,11 @@ constexpr int kGenMaxDim = 256;
 struct GenericParams {
     const void* q;          // fp32 or fp16
     void* out;              // fp32 or fp16
-    const __half* k;        // cache: contiguous [batch, Hkv, kv_stride, D] or pool [num_blocks*bs, Hkv, D]
-    const __half* v;
+    const void* k;          // cache: contiguous [batch, Hkv, kv_stride, D] or pool [num_blocks*bs, Hkv, D]
+    const void* v;
+    const float* k_scales;  // 8-bit pools: [num_blocks, Hkv]
+    const float* v_scales;
+    int window, sinks;      // window 0: none
     const __half* k_tree;   // [batch, Hkv, N, D] or nullptr
     const __half* v_tree;
     const int* tables;      // [batch, max_blocks] or nullptr (contiguous)
@@ -58,10 +66,24 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
     return m;
 }
 
+template <int kElem>
+struct CacheElem { using type = uint8_t; };
+template <>
+struct CacheElem<kElemF16> { using type = __half; };
+
+template <int kElem>
+__device__ __forceinline__ float to_float(typename CacheElem<kElem>::type x) {
+    if constexpr (kElem == kElemF16) return __half2float(x);
+    else if constexpr (kElem == kElemInt8) return (float)(int8_t)x;
+    else return __half2float(__half(__nv_cvt_fp8_to_halfraw(x, __NV_E4M3)));
+}
+
+template <int kElem, bool kWindow>
 __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericParams p) {
+    using T = typename CacheElem<kElem>::type;
     __shared__ float s_q[kGenMaxDim];
     __shared__ float s_p[kGenThreads];
-    __shared__ const __half* s_vrow[kGenThreads];
+    __shared__ const T* s_vrow[kGenThreads];
     __shared__ float s_red[kGenThreads / 32];
     const int tid = threadIdx.x;
     const int h = blockIdx.y;
@@ -81,6 +103,13 @@ __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericP
     }
     int visible = cache_len;  // cache keys [0, visible)
     if (p.causal_start >= 0) visible = min(cache_len, p.causal_start + r + 1);
+    int gap = 0, sinks_end = 0;  // list entry i is key i before sinks_end, key i + gap from there on
+    if constexpr (kWindow) {
+        const WindowSpan w = window_span(p.causal_start >= 0 ? p.causal_start + r : cache_len - 1, p.window, p.sinks);
+        sinks_end = min(w.sinks_end, visible);
+        gap = max(min(w.lo, visible) - sinks_end, 0);
+        visible -= gap;
+    }
     // tree part: the node's own key and its ancestors' (bit j of the word)
     unsigned long long anc = 0ull;
     if (p.parents) {
@@ -101,9 +130,11 @@ __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericP
     float acc[kGenMaxDim / kGenThreads] = {0.f, 0.f};  // output dims tid, tid + 128
     for (int base = 0; base < total; base += kGenThreads) {
         // phase 1: thread = key
-        const int key = base + tid;
-        const __half *krow = nullptr, *vrow = nullptr;
-        if (key < visible) {
+        const int entry = base + tid;
+        const int key = kWindow && entry >= sinks_end ? entry + gap : entry;
+        const T *krow = nullptr, *vrow = nullptr;
+        float k_scale = 1.f, v_scale = 1.f;
+        if (entry < visible) {
             size_t row;
             bool ok = true;
             if (p.tables) {
@@ -117,20 +148,42 @@ __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericP
                 row = ((size_t)b * p.hkv + kvh) * p.kv_stride + key;
             }
             if (ok) {
-                krow = p.k + row * p.d;
-                vrow = p.v + row * p.d;
+                krow = static_cast<const T*>(p.k) + row * p.d;
+                vrow = static_cast<const T*>(p.v) + row * p.d;
+                if constexpr (kElem != kElemF16) {
+                    const size_t page = row / ((size_t)p.hkv * p.block_size) * p.hkv + kvh;
+                    k_scale = p.k_scales[page];
+                    v_scale = p.v_scales[page];
+                }
             }
-        } else if (key < total) {
-            const int node = key - visible;
-            if ((anc >> node) & 1ull) {
-                const size_t row = ((size_t)b * p.hkv + kvh) * p.n_nodes + node;
-                krow = p.k_tree + row * p.d;
-                vrow = p.v_tree + row * p.d;
+        } else if (entry < total) {
+            if constexpr (kElem == kElemF16 && !kWindow) {
+                const int node = entry - visible;
+                if ((anc >> node) & 1ull) {
+                    const size_t row = ((size_t)b * p.hkv + kvh) * p.n_nodes + node;
+                    krow = p.k_tree + row * p.d;
+                    vrow = p.v_tree + row * p.d;
+                }
             }
         }
         float s = -INFINITY;
         if (krow) {
             float dot = 0.f;
+            if constexpr (kElem != kElemF16) {
+                for (int i = 0; i < p.d; i += 8) {  // 8-byte pieces
+                    const uint2 pk = *reinterpret_cast<const uint2*>(krow + i);
+                    const float4 a = q8_decode4<kElem>(pk.x), b4 = q8_decode4<kElem>(pk.y);
+                    dot = fmaf(s_q[i], a.x, dot);
+                    dot = fmaf(s_q[i + 1], a.y, dot);
+                    dot = fmaf(s_q[i + 2], a.z, dot);
+                    dot = fmaf(s_q[i + 3], a.w, dot);
+                    dot = fmaf(s_q[i + 4], b4.x, dot);
+                    dot = fmaf(s_q[i + 5], b4.y, dot);
+                    dot = fmaf(s_q[i + 6], b4.z, dot);
+                    dot = fmaf(s_q[i + 7], b4.w, dot);
+                }
+                dot *= k_scale;
+            } else
             for (int i = 0; i < p.d; i += 8) {  // head_dim is a multiple of 8: 16-byte pieces
                 const uint4 pk = *reinterpret_cast<const uint4*>(krow + i);
                 const __half2* h2 = reinterpret_cast<const __half2*>(&pk);
@@ -146,7 +199,7 @@ __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericP
         const float m_chunk = block_max(s, s_red);
         const float m_new = fmaxf(m_run, m_chunk);
         const float pw = (krow && m_new > -INFINITY) ? __expf(s - m_new) : 0.f;
-        s_p[tid] = pw;
+        s_p[tid] = kElem == kElemF16 ? pw : pw * v_scale;
         s_vrow[tid] = vrow;
         const float l_chunk = block_sum(pw, s_red);  // its barriers also publish s_p / s_vrow
         const float alpha = m_run > -INFINITY ? __expf(m_run - m_new) : 0.f;
@@ -160,8 +213,8 @@ __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericP
             if (dim >= p.d) continue;
             float a = acc[u] * alpha;
             for (int j = 0; j < n_keys; j++) {
-                const __half* vr = s_vrow[j];
-                if (vr) a = fmaf(s_p[j], __half2float(vr[dim]), a);
+                const T* vr = s_vrow[j];
+                if (vr) a = fmaf(s_p[j], to_float<kElem>(vr[dim]), a);
             }
             acc[u] = a;
         }
@@ -177,7 +230,7 @@ __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericP
     }
 }
 
-int launch(granite_cuda_compute* c, const GenericParams& p, const char* name) {
+int launch(granite_cuda_compute* c, const GenericParams& p, const char* name, int elem = kElemF16) {
     if (p.d <= 0 || p.d > kGenMaxDim || p.d % 8 != 0)
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, std::string(name) + ": head_dim must be a multiple of 8, at most 256");
     if (p.hkv <= 0 || p.hq % p.hkv != 0)
@@ -186,14 +239,27 @@ int launch(granite_cuda_compute* c, const GenericParams& p, const char* name) {
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, std::string(name) + ": too many query rows or heads for one launch");
     if (p.batch == 0 || p.q_rows == 0) return GRANITE_CUDA_SUCCESS;
     LaunchScope t(c, name);
-    generic_attention_kernel<<<dim3((unsigned)(p.batch * p.q_rows), (unsigned)p.hq), kGenThreads, 0, c->stream>>>(p);
+    auto kern = elem == kElemInt8   ? generic_attention_kernel<kElemInt8, true>  // the 8-bit builds take window 0 too
+                : elem == kElemE4M3 ? generic_attention_kernel<kElemE4M3, true>
+                : p.window > 0      ? generic_attention_kernel<kElemF16, true>
+                                    : generic_attention_kernel<kElemF16, false>;
+    kern<<<dim3((unsigned)(p.batch * p.q_rows), (unsigned)p.hq), kGenThreads, 0, c->stream>>>(p);
     GB_CUDA_TRY(cudaGetLastError());
     return GRANITE_CUDA_SUCCESS;
 }
 
+// The window and scales of a call; windows are kept in the range that positions have.
+void set_view(GenericParams& p, const CacheView& view) {
+    p.k_scales = view.k_scales;
+    p.v_scales = view.v_scales;
+    p.window = (int)(view.window < 0x7fffffffu ? view.window : 0x7fffffffu);
+    p.sinks = (int)(view.sinks < 0x7fffffffu ? view.sinks : 0x7fffffffu);
+}
+
 }  // namespace
 
-int launch_generic_decode(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq) {
+int launch_generic_decode(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq,
+                          const CacheView& view) {
     if (!a.q || !a.k_cache || !a.v_cache || !a.output || (!contiguous && !a.block_tables))
         return fail(GRANITE_CUDA_NULL_POINTER, "decode: null buffer");
     if (!contiguous && (a.block_size == 0 || a.num_blocks == 0 || a.max_blocks_per_seq == 0))
@@ -201,8 +267,8 @@ int launch_generic_decode(granite_cuda_compute* c, const GraniteCudaPagedDecodeA
     GenericParams p{};
     p.q = a.q;
     p.out = a.output;
-    p.k = static_cast<const __half*>(a.k_cache);
-    p.v = static_cast<const __half*>(a.v_cache);
+    p.k = a.k_cache;
+    p.v = a.v_cache;
     p.tables = contiguous ? nullptr : a.block_tables;
     p.kv_lens = a.seq_lens;
     p.batch = (int)a.batch_size;
@@ -218,10 +284,11 @@ int launch_generic_decode(granite_cuda_compute* c, const GraniteCudaPagedDecodeA
     p.causal_start = -1;
     p.scale = a.scale;
     p.status = c->d_status;
-    return launch(c, p, "generic_decode");
+    set_view(p, view);
+    return launch(c, p, "generic_decode", view.elem);
 }
 
-int launch_generic_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a) {
+int launch_generic_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, const CacheView& view) {
     if (!a.q || !a.k || !a.v || !a.output) return fail(GRANITE_CUDA_NULL_POINTER, "prefill: null buffer");
     if (a.q_dtype > 1 || a.out_dtype > 1) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "prefill: dtype must be 0 (fp32) or 1 (fp16)");
     const uint32_t max_seq = a.max_seq ? a.max_seq : a.seq_kv;
@@ -231,8 +298,8 @@ int launch_generic_prefill(granite_cuda_compute* c, const GraniteCudaAttentionAr
     p.out = a.output;
     p.q_f16 = a.q_dtype == 1;
     p.out_f16 = a.out_dtype == 1;
-    p.k = static_cast<const __half*>(a.k);
-    p.v = static_cast<const __half*>(a.v);
+    p.k = a.k;
+    p.v = a.v;
     p.batch = a.batch_size ? (int)a.batch_size : 1;
     p.q_rows = (int)a.seq_q;
     p.hq = (int)a.num_heads;
@@ -243,10 +310,11 @@ int launch_generic_prefill(granite_cuda_compute* c, const GraniteCudaAttentionAr
     p.causal_start = (int)a.start_pos;
     p.scale = a.scale;
     p.status = c->d_status;
-    return launch(c, p, "generic_prefill");
+    set_view(p, view);
+    return launch(c, p, "generic_prefill", view.elem);
 }
 
-int launch_generic_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a) {
+int launch_generic_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a, const CacheView& view) {
     if (!a.q || !a.k_cache || !a.v_cache || !a.block_table || !a.output)
         return fail(GRANITE_CUDA_NULL_POINTER, "paged_prefill_attention: null buffer");
     if (a.q_dtype > 1 || a.out_dtype > 1)
@@ -260,8 +328,8 @@ int launch_generic_paged_prefill(granite_cuda_compute* c, const GraniteCudaPaged
     p.out = a.output;
     p.q_f16 = a.q_dtype == 1;
     p.out_f16 = a.out_dtype == 1;
-    p.k = static_cast<const __half*>(a.k_cache);
-    p.v = static_cast<const __half*>(a.v_cache);
+    p.k = a.k_cache;
+    p.v = a.v_cache;
     p.tables = a.block_table;
     p.batch = 1;
     p.q_rows = (int)a.seq_q;
@@ -275,7 +343,8 @@ int launch_generic_paged_prefill(granite_cuda_compute* c, const GraniteCudaPaged
     p.causal_start = (int)a.start_pos;
     p.scale = a.scale;
     p.status = c->d_status;
-    return launch(c, p, "generic_paged_prefill");
+    set_view(p, view);
+    return launch(c, p, "generic_paged_prefill", view.elem);
 }
 
 int launch_generic_tree(granite_cuda_compute* c, const GraniteCudaTreeAttentionArgs& a) {
@@ -296,8 +365,8 @@ int launch_generic_tree(granite_cuda_compute* c, const GraniteCudaTreeAttentionA
     p.out = a.output;
     p.q_f16 = a.q_dtype == 1;
     p.tree_layout = 1;
-    p.k = static_cast<const __half*>(a.k_cache);
-    p.v = static_cast<const __half*>(a.v_cache);
+    p.k = a.k_cache;
+    p.v = a.v_cache;
     p.k_tree = static_cast<const __half*>(a.k_tree);
     p.v_tree = static_cast<const __half*>(a.v_tree);
     p.tables = a.block_tables;

@@ -1,0 +1,247 @@
+// RoPE fused with the write into the 8-bit paged cache.
+//
+// For a page that the call touches, for one KV head and for K (rotated) or V, with x the call's rows in the page:
+//     need = max |x| / qmax        scale' = max(need, scale of the page's older rows; 0 when row 0 is new)
+//     new rows: round(x / scale')  older rows: round(code * (scale / scale')), only when the scale grew
+// The rotation and its roundings are those of the fp16 append (rope_append.cu): adjacent pairs, tables from the
+// host, both products rounded separately.  Divisions are IEEE divisions: a code then depends on nothing but the
+// formula above, so the same inputs give the same bytes whatever the batch around them.
+//
+// One warp per (sequence, touched page, KV head, K or V): the scale needs the whole page before the first
+// code can be written, and a page of one head is 16 rows x head_dim, which a warp holds in registers (16 float4 per
+// lane for head_dim 128) - every input is read once, a row is one 512-byte load and one 128-byte store.  The
+// older rows are only touched when the scale grows.  Query heads are rotated by further blocks of the same launch, four
+// 16-byte pieces per thread.  Bound by HBM for chunks (Q is read and written in 32 bits: three quarters of the bytes),
+// by the chain position -> table entry -> scale -> older rows for a decode step.
+#include "compute_internal.h"
+#include "ptx.cuh"
+#include "q8.cuh"
+
+namespace gb200 {
+
+namespace {
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kQueryPieces = 4;  // 16-byte pieces of Q per thread
+
+struct Q8AppendParams {
+    float* q;
+    const float* k;
+    const float* v;
+    const float* cos_t;
+    const float* sin_t;
+    uint8_t* k_pool;
+    uint8_t* v_pool;
+    float* k_scales;
+    float* v_scales;
+    const int* tables;
+    const int* positions;
+    int batch, new_len, hq, hkv, head_dim, block_size, max_blocks, num_blocks, table_len, start_pos;
+    int pages_per_seq;      // touched pages of a sequence at most
+    long long page_blocks;  // blocks that write pages; the blocks behind them rotate Q
+    int blocks_per_token;   // of the Q rotation
+    int* status;
+};
+
+__device__ __forceinline__ float4 rotate_quad(float4 x, float2 c, float2 s) {
+    float4 r;
+    r.x = __fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(x.y, s.x));
+    r.y = __fadd_rn(__fmul_rn(x.x, s.x), __fmul_rn(x.y, c.x));
+    r.z = __fsub_rn(__fmul_rn(x.z, c.y), __fmul_rn(x.w, s.y));
+    r.w = __fadd_rn(__fmul_rn(x.z, s.y), __fmul_rn(x.w, c.y));
+    return r;
+}
+__device__ __forceinline__ float max_abs(float4 x) { return fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))); }
+__device__ __forceinline__ bool drop_non_finite(float& x) {
+    if (fabsf(x) < INFINITY) return false;
+    x = 0.f;
+    return true;
+}
+__device__ __forceinline__ float4 over(float4 x, float scale) {
+    return make_float4(__fdiv_rn(x.x, scale), __fdiv_rn(x.y, scale), __fdiv_rn(x.z, scale), __fdiv_rn(x.w, scale));
+}
+
+// kQuads: float4 pieces of a head row for head_dim 128 (32) and 64 (16) with 16-token pages, the rows then stay in
+// registers; 0: any other shape, whose rows are read twice (the second time from the caches).
+template <int kElem, int kQuads>
+__global__ void __launch_bounds__(kAppendThreads) q8_append_kernel(const __grid_constant__ Q8AppendParams p) {
+    const int lane = threadIdx.x & 31;
+    const int quads = kQuads ? kQuads : p.head_dim / 4;
+    if (blockIdx.x >= p.page_blocks) {
+        // ---- rotate Q in place
+        const long long blk = blockIdx.x - p.page_blocks;
+        const long long token = blk / p.blocks_per_token;
+        const int first = (int)(blk - token * p.blocks_per_token) * kAppendThreads * kQueryPieces + threadIdx.x;
+        const int b = (int)(token / p.new_len), s = (int)(token - (long long)b * p.new_len);
+        const long long pos = (long long)(p.positions ? p.positions[b] : p.start_pos) + s;
+        if (pos < 0 || pos >= p.table_len) return;  // reported by the page blocks
+        float4* row = reinterpret_cast<float4*>(p.q) + token * p.hq * quads;
+        const int n = p.hq * quads;
+        float4 x[kQueryPieces];
+#pragma unroll
+        for (int j = 0; j < kQueryPieces; j++)
+            if (first + j * kAppendThreads < n) x[j] = row[first + j * kAppendThreads];
+#pragma unroll
+        for (int j = 0; j < kQueryPieces; j++) {
+            const int i = first + j * kAppendThreads;
+            if (i >= n) break;
+            const size_t trig = (size_t)pos * (p.head_dim / 2) + 2 * (i % quads);
+            row[i] = rotate_quad(x[j], *reinterpret_cast<const float2*>(p.cos_t + trig), *reinterpret_cast<const float2*>(p.sin_t + trig));
+        }
+        return;
+    }
+
+    // ---- one page of one head: task = ((sequence, page), head, K or V)
+    long long task = (long long)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
+    const bool is_v = task & 1;
+    task >>= 1;
+    const int h = (int)(task % p.hkv);
+    task /= p.hkv;
+    const int pi = (int)(task % p.pages_per_seq);
+    const long long b = task / p.pages_per_seq;
+    if (b >= p.batch) return;
+    const int start = p.positions ? p.positions[b] : p.start_pos;
+    const long long room = min((long long)p.table_len, (long long)p.max_blocks * p.block_size);
+    const int lo = max(start, 0);
+    const int hi = (int)min((long long)start + p.new_len, room);
+    if (pi == 0 && h == 0 && !is_v && lane == 0 && (start < 0 || (long long)start + p.new_len > room))
+        atomicOr(p.status, kStatusBadSeqLen);
+    const int logical = lo / p.block_size + pi;
+    const long long page0 = (long long)logical * p.block_size;  // position of the page's row 0
+    const int r0 = (int)max(lo - page0, 0LL), r1 = (int)min(hi - page0, (long long)p.block_size);
+    if (r0 >= r1) return;
+    const int phys = p.tables[(size_t)b * p.max_blocks + logical];
+    if (phys < 0 || phys >= p.num_blocks) {
+        if (lane == 0) atomicOr(p.status, kStatusBadTable);
+        return;
+    }
+    const float4* src = reinterpret_cast<const float4*>(is_v ? p.v : p.k);
+    uint32_t* pool = reinterpret_cast<uint32_t*>(is_v ? p.v_pool : p.k_pool);
+    float* scales = (is_v ? p.v_scales : p.k_scales) + (size_t)phys * p.hkv + h;
+    const float before = r0 > 0 ? *scales : 0.f;
+
+    bool dropped = false;
+    auto fetch = [&](int i) {  // piece i of the page: row i / quads
+        const int row = i / quads, u = i - row * quads;
+        const long long s = page0 + row - start;  // which of the call's tokens
+        float4 x = src[(((size_t)b * p.new_len + s) * p.hkv + h) * quads + u];
+        if (!is_v) {
+            const size_t trig = (size_t)(page0 + row) * (p.head_dim / 2) + 2 * u;
+            x = rotate_quad(x, *reinterpret_cast<const float2*>(p.cos_t + trig), *reinterpret_cast<const float2*>(p.sin_t + trig));
+        }
+        dropped |= drop_non_finite(x.x) | drop_non_finite(x.y) | drop_non_finite(x.z) | drop_non_finite(x.w);
+        return x;
+    };
+    auto word = [&](int i) {  // where the codes of piece i live
+        const int row = i / quads, u = i - row * quads;
+        return pool + (((size_t)phys * p.block_size + row) * p.hkv + h) * quads + u;
+    };
+    const int i0 = r0 * quads, i1 = r1 * quads;
+    float amax = 0.f;
+    constexpr int kIts = kQuads ? 16 * kQuads / 32 : 1;
+    float4 held[kIts];
+    if (kQuads) {
+#pragma unroll
+        for (int it = 0; it < kIts; it++) {
+            const int i = it * 32 + lane;
+            if (i >= i0 && i < i1) held[it] = fetch(i);
+            else held[it] = make_float4(0.f, 0.f, 0.f, 0.f);
+            amax = fmaxf(amax, max_abs(held[it]));
+        }
+    } else {
+        for (int i = i0 + lane; i < i1; i += 32) amax = fmaxf(amax, max_abs(fetch(i)));
+    }
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, sh));
+    float need = __fdiv_rn(amax, q8_max<kElem>());
+    if (need < 1.17549435e-38f) need = 0.f;  // below the normal range: stored as zeros
+    const float scale = fmaxf(before, need);
+    if (dropped) atomicOr(p.status, kStatusNonFinite);
+
+    if (scale > before && r0 > 0) {
+        const float ratio = __fdiv_rn(before, scale);
+        for (int i = lane; i < i0; i += 32) {
+            const float4 x = q8_decode4<kElem>(*word(i));
+            *word(i) = q8_encode4<kElem>(make_float4(__fmul_rn(x.x, ratio), __fmul_rn(x.y, ratio), __fmul_rn(x.z, ratio), __fmul_rn(x.w, ratio)));
+        }
+    }
+    if (kQuads) {
+#pragma unroll
+        for (int it = 0; it < kIts; it++) {
+            const int i = it * 32 + lane;
+            if (i >= i0 && i < i1) *word(i) = scale > 0.f ? q8_encode4<kElem>(over(held[it], scale)) : 0u;
+        }
+    } else {
+        for (int i = i0 + lane; i < i1; i += 32) *word(i) = scale > 0.f ? q8_encode4<kElem>(over(fetch(i), scale)) : 0u;
+    }
+    if (lane == 0) *scales = scale;
+}
+
+}  // namespace
+
+int check_q8_append(const GraniteCudaRopeAppendArgs& a, const GraniteCudaQ8Cache& x) {
+    if (!a.k || !a.v || !a.cos_table || !a.sin_table || !a.k_cache || !a.v_cache || !a.block_tables || !x.k_scales || !x.v_scales)
+        return fail(GRANITE_CUDA_NULL_POINTER, "rope_paged_kv_cache_append_q8: null buffer");
+    if (x.cache_dtype > 1) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "rope_paged_kv_cache_append_q8: cache_dtype must be 0 (int8) or 1 (e4m3)");
+    if (a.batch_size == 0 || a.new_len == 0) return GRANITE_CUDA_SUCCESS;
+    if (a.head_dim == 0 || a.head_dim % 8 != 0 || a.head_dim > 256)
+        return fail(GRANITE_CUDA_INVALID_ARGUMENT, "rope_paged_kv_cache_append_q8: head_dim must be a multiple of 8, at most 256");
+    if (a.num_kv_heads == 0 || a.block_size == 0 || a.num_blocks == 0 || a.max_blocks_per_seq == 0 || (a.q && a.num_heads == 0))
+        return fail(GRANITE_CUDA_INVALID_ARGUMENT, "rope_paged_kv_cache_append_q8: empty shape");
+    const uintptr_t align16 = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                              reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache);
+    if (align16 & 15) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "rope_paged_kv_cache_append_q8: Q, K, V and the pools must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(a.cos_table) | reinterpret_cast<uintptr_t>(a.sin_table)) & 7)
+        return fail(GRANITE_CUDA_INVALID_ARGUMENT, "rope_paged_kv_cache_append_q8: the RoPE tables must be 8-byte aligned");
+    const uint64_t limit = 1ull << 31;
+    if (a.batch_size >= limit || a.new_len >= limit || a.num_heads > 65535 || a.num_kv_heads > 65535 || a.block_size >= limit ||
+        a.max_blocks_per_seq >= limit || a.num_blocks >= limit || a.table_len >= limit || a.start_pos >= limit)
+        return fail(GRANITE_CUDA_INVALID_ARGUMENT, "rope_paged_kv_cache_append_q8: a size is out of range (65535 heads, 2^31 - 1 otherwise)");
+    return GRANITE_CUDA_SUCCESS;
+}
+
+int launch_q8_append(granite_cuda_compute* c, const GraniteCudaRopeAppendArgs& a, const GraniteCudaQ8Cache& x) {
+    if (a.batch_size == 0 || a.new_len == 0) return GRANITE_CUDA_SUCCESS;
+    Q8AppendParams p{};
+    p.q = a.q;
+    p.k = a.k;
+    p.v = a.v;
+    p.cos_t = a.cos_table;
+    p.sin_t = a.sin_table;
+    p.k_pool = static_cast<uint8_t*>(a.k_cache);
+    p.v_pool = static_cast<uint8_t*>(a.v_cache);
+    p.k_scales = x.k_scales;
+    p.v_scales = x.v_scales;
+    p.tables = a.block_tables;
+    p.positions = a.positions;
+    p.batch = (int)a.batch_size;
+    p.new_len = (int)a.new_len;
+    p.hq = a.q ? (int)a.num_heads : 0;
+    p.hkv = (int)a.num_kv_heads;
+    p.head_dim = (int)a.head_dim;
+    p.block_size = (int)a.block_size;
+    p.max_blocks = (int)a.max_blocks_per_seq;
+    p.num_blocks = (int)a.num_blocks;
+    p.table_len = (int)a.table_len;
+    p.start_pos = (int)a.start_pos;
+    p.status = c->d_status;
+    p.pages_per_seq = (int)(((uint64_t)a.new_len + a.block_size - 2) / a.block_size) + 1;
+    const uint64_t tasks = (uint64_t)a.batch_size * p.pages_per_seq * a.num_kv_heads * 2;
+    p.page_blocks = (long long)((tasks + kAppendWarps - 1) / kAppendWarps);
+    const uint64_t per_block = kAppendThreads * kQueryPieces;
+    p.blocks_per_token = (int)(((uint64_t)p.hq * (a.head_dim / 4) + per_block - 1) / per_block);
+    const uint64_t grid = (uint64_t)p.page_blocks + (uint64_t)a.batch_size * a.new_len * p.blocks_per_token;
+    if (grid >= (1ull << 31)) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "rope_paged_kv_cache_append_q8: too many tokens for one call");
+    const int quads = a.block_size == 16 ? (a.head_dim == 128 ? 32 : a.head_dim == 64 ? 16 : 0) : 0;
+    const bool e4m3 = x.cache_dtype == GRANITE_CUDA_CACHE_E4M3;
+    auto kern = quads == 32   ? (e4m3 ? q8_append_kernel<kElemE4M3, 32> : q8_append_kernel<kElemInt8, 32>)
+                : quads == 16 ? (e4m3 ? q8_append_kernel<kElemE4M3, 16> : q8_append_kernel<kElemInt8, 16>)
+                              : (e4m3 ? q8_append_kernel<kElemE4M3, 0> : q8_append_kernel<kElemInt8, 0>);
+    LaunchScope t(c, "rope_paged_kv_append_q8");
+    kern<<<(unsigned)grid, kAppendThreads, 0, c->stream>>>(p);
+    GB_CUDA_TRY(cudaGetLastError());
+    return GRANITE_CUDA_SUCCESS;
+}
+
+}  // namespace gb200

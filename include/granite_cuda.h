@@ -452,6 +452,63 @@ typedef struct {
 
 int granite_cuda_paged_prefill_attention(granite_cuda_compute_t* c, const GraniteCudaPagedPrefillArgs* args);
 
+/* ---- 8-bit paged K/V cache ---------------------------------------------------------------------------
+ * Half the bytes of the fp16 pool: K and V are held as 8-bit codes [num_blocks*block_size,
+ * num_kv_heads, head_dim] with one fp32 scale per (page, KV head), k_scales / v_scales
+ * [num_blocks, num_kv_heads]; code * scale is the value a code stands for.  cache_dtype 0: int8 codes in
+ * [-127, 127]; 1: fp8 e4m3 codes in [-448, 448].  The addressing rule, block tables and page size are those of the
+ * fp16 pool.  Pools must be 16-byte aligned.  No reference counterpart (the reference caches fp16). */
+enum { GRANITE_CUDA_CACHE_INT8 = 0, GRANITE_CUDA_CACHE_E4M3 = 1 };
+
+typedef struct {
+    float* k_scales;      /* [num_blocks, num_kv_heads] fp32, device */
+    float* v_scales;
+    uint32_t cache_dtype; /* GRANITE_CUDA_CACHE_INT8 or GRANITE_CUDA_CACHE_E4M3 */
+} GraniteCudaQ8Cache;
+
+/* A sliding window: the query at position p sees key j <= p when p - j < window or j < sinks (the first few
+ * tokens, kept visible).  window 0 is refused; a window that covers the whole sequence hides nothing. */
+typedef struct {
+    uint32_t window;
+    uint32_t sinks;
+} GraniteCudaAttentionWindow;
+
+/* granite_cuda_rope_paged_kv_cache_append into the 8-bit cache (args->k_cache / v_cache are its pools).  For every
+ * (sequence, page the call touches, KV head), for K after the rotation and for V:
+ *     need  = max |x| over the call's rows in the page / (127 or 448)
+ *     scale = max(need, the page's scale before the call)    - or need alone when the call writes the page's row 0
+ *     new rows:   code = round(x / scale)                    - round to nearest even
+ *     older rows: code = round(code * (scale before / scale)), unchanged when the scale did not grow
+ * Rows behind the call's last are left as they are.  A scale below 2^-126 is stored as 0 with zero codes.  A NaN or
+ * infinite K or V value does not enter the maximum, is stored as 0 and reported by granite_cuda_sync as
+ * InvalidArgument.  A page that this call writes must belong to one sequence only (pages shared by several sequences
+ * may be read by any number of them); a token that cannot be placed is skipped and reported as by the fp16 call.
+ * head_dim: a multiple of 8, at most 256; any block_size. */
+int granite_cuda_rope_paged_kv_cache_append_q8(granite_cuda_compute_t* c, const GraniteCudaRopeAppendArgs* args,
+                                               const GraniteCudaQ8Cache* cache);
+
+/* granite_cuda_batched_paged_attention_decode over the 8-bit cache; window may be NULL.  Tuned kernel: head_dim 128
+ * or 64, block_size 16; other head dims (multiples of 8 up to 256) and page sizes run on a plain fp32 kernel.  Codes
+ * and scales are not rounded on the way: results have the accuracy of fp32 arithmetic on the values held. */
+int granite_cuda_batched_paged_attention_decode_q8(granite_cuda_compute_t* c, const GraniteCudaPagedDecodeArgs* args,
+                                                   const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window);
+
+/* granite_cuda_paged_prefill_attention over the 8-bit cache; window may be NULL.  Same shapes as the fp16 call. */
+int granite_cuda_paged_prefill_attention_q8(granite_cuda_compute_t* c, const GraniteCudaPagedPrefillArgs* args,
+                                            const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window);
+
+/* ---- sliding window with sinks over the fp16 caches --------------------------------------------------------
+ * The three calls without the suffix, restricted to the keys that the window leaves visible.  A sequence's query
+ * positions are those of the plain calls (decode: the last token; prefill: start_pos + i).  Pages that no query of the
+ * call sees are not read and their table entries are not looked at, so a host may free them.  A query row that sees no
+ * key at all (contiguous prefill with seq_kv short of the window's start) gets zeros. */
+int granite_cuda_batched_paged_attention_decode_window(granite_cuda_compute_t* c, const GraniteCudaPagedDecodeArgs* args,
+                                                       const GraniteCudaAttentionWindow* window);
+int granite_cuda_multihead_attention_window(granite_cuda_compute_t* c, const GraniteCudaAttentionArgs* args,
+                                            const GraniteCudaAttentionWindow* window);
+int granite_cuda_paged_prefill_attention_window(granite_cuda_compute_t* c, const GraniteCudaPagedPrefillArgs* args,
+                                                const GraniteCudaAttentionWindow* window);
+
 /* ---- output gather over NVLink peer memory ---------------------------------------------------------
  * Sequences are sharded across GPUs with no exchange inside attention; what follows the path is a
  * gather of the per-GPU output rows.  This call pushes `bytes` bytes from `src` (this GPU) to
