@@ -1,6 +1,7 @@
 // Attention calls that see the cache through a view - 8-bit codes with page scales, a sliding window, or both: their
 // argument checks (none of which needs a device) and the choice between the tuned and the plain kernel.
 #include "compute_internal.h"
+#include "q8.cuh"
 
 namespace gb200 {
 
@@ -73,7 +74,9 @@ int check_paged_prefill_view(const GraniteCudaPagedPrefillArgs& a) {
 
 int launch_decode_view(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq, const CacheView& view) {
     if (a.batch_size == 0) return GRANITE_CUDA_SUCCESS;
-    return launch_generic_decode(c, a, contiguous, max_seq, view);
+    if (view.elem == kElemInt8) return launch_paged_decode_int8(c, a, view);
+    if (view.elem == kElemE4M3) return launch_paged_decode_e4m3(c, a, view);
+    return launch_paged_decode_window(c, a, contiguous, max_seq, view);
 }
 
 int launch_prefill_view(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, const CacheView& view) {

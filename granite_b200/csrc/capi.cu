@@ -148,6 +148,16 @@ const CUtensorMap* granite_cuda_compute::tensor_map_page_groups(const void* base
     return encode_map(key);
 }
 
+const CUtensorMap* granite_cuda_compute::tensor_map_pages_q8(const void* base, uint32_t head_dim, uint64_t rows, uint64_t heads,
+                                                             uint32_t rows_per_box, uint32_t tile_heads) {
+    // (bytes seen as pairs: a row of head_dim bytes is head_dim / 2 halfs)
+    TensorMapKey key{base, head_dim / 2, rows, 1, heads * head_dim, 128, head_dim / 2, rows_per_box, 1, (int)head_dim, 4};
+    key.dim3 = heads;
+    key.stride3 = head_dim;
+    key.box3 = tile_heads;
+    return encode_map(key);
+}
+
 cudaEvent_t granite_cuda_compute::take_event() {
     if (!event_pool.empty()) {
         cudaEvent_t e = event_pool.back();

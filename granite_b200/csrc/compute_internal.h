@@ -114,6 +114,10 @@ struct granite_cuda_compute {
     // 8 rows, 64-wide chunks of a head, rows / 8}, box {64, 8, all chunks, 2} = one 16-row page of one
     // head, landing as [row group][chunk][8 rows][64]; x selects the head (x = head * head_dim).
     const CUtensorMap* tensor_map_page_groups(const void* base, uint64_t width, uint64_t rows, uint32_t head_dim);
+    // The 8-bit pool [rows, heads, head_dim] (head_dim 128 or 64): box {one head's row, 16 rows, tile_heads heads}, landing as
+    // [head][row][head_dim bytes] under a swizzle as wide as the row.
+    const CUtensorMap* tensor_map_pages_q8(const void* base, uint32_t head_dim, uint64_t rows, uint64_t heads, uint32_t rows_per_box,
+                                           uint32_t tile_heads);
     const CUtensorMap* encode_map(const gb200::TensorMapKey& key);
 };
 
@@ -164,6 +168,9 @@ struct CacheView {
     const float* v_scales = nullptr;
     uint32_t window = 0, sinks = 0;
 };
+int launch_paged_decode_int8(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, const CacheView& view);
+int launch_paged_decode_e4m3(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, const CacheView& view);
+int launch_paged_decode_window(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq, const CacheView& view);
 // plain fp32 kernel for head dims, page sizes and head counts outside the tuned kernels' shapes
 int launch_generic_decode(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq,
                           const CacheView& view = CacheView{});
