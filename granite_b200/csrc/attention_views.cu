@@ -7,7 +7,7 @@ namespace gb200 {
 
 namespace {
 
-constexpr uint64_t kIntLimit = 1ull << 31;
+constexpr uint64_t kIntLimit = (1ull << 31) - 65536;  // positions and rows, with room for a tile more in int arithmetic
 
 bool unaligned16(const void* a, const void* b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) != 0; }
 
@@ -22,7 +22,7 @@ int check_heads(uint32_t num_heads, uint32_t num_kv_heads, uint32_t head_dim, co
 int check_pool(uint32_t block_size, uint32_t num_blocks, uint32_t max_blocks, const std::string& what) {
     if (block_size == 0 || num_blocks == 0 || max_blocks == 0) return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": empty pool or table");
     if ((uint64_t)block_size * max_blocks >= kIntLimit || (uint64_t)block_size * num_blocks >= kIntLimit)
-        return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": the pool or a block table spans 2^31 tokens or more");
+        return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": the pool or a block table spans about 2^31 tokens or more");
     return GRANITE_CUDA_SUCCESS;
 }
 
@@ -81,12 +81,12 @@ int launch_decode_view(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs
 
 int launch_prefill_view(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, const CacheView& view) {
     if (a.seq_q == 0) return GRANITE_CUDA_SUCCESS;
-    return launch_generic_prefill(c, a, view);
+    return launch_prefill(c, a, view);
 }
 
 int launch_paged_prefill_view(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a, const CacheView& view) {
     if (a.seq_q == 0) return GRANITE_CUDA_SUCCESS;
-    return launch_generic_paged_prefill(c, a, view);
+    return view.elem != kElemF16 ? launch_paged_prefill_q8(c, a, view) : launch_paged_prefill(c, a, view);
 }
 
 }  // namespace gb200

@@ -149,7 +149,15 @@ struct DecodeGather {
 };
 int launch_paged_decode(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous,
                         uint32_t max_seq, const DecodeGather* gather = nullptr);
-int launch_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a);
+// What distinguishes an 8-bit or windowed attention call from the plain one: the cache's element type and scales (elem as
+// in q8.cuh: 0 fp16, 1 int8, 2 e4m3) and the window (0: none).
+struct CacheView {
+    int elem = 0;
+    const float* k_scales = nullptr;
+    const float* v_scales = nullptr;
+    uint32_t window = 0, sinks = 0;
+};
+int launch_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, const CacheView& view = CacheView{});
 int launch_tree_verify(granite_cuda_compute* c, const GraniteCudaTreeAttentionArgs& a);
 int launch_kv_cache_append(granite_cuda_compute* c, const GraniteCudaKvAppendArgs& a);
 int launch_paged_kv_cache_append(granite_cuda_compute* c, const GraniteCudaPagedKvAppendArgs& a);
@@ -159,15 +167,8 @@ int launch_rope_multihead(granite_cuda_compute* c, float* q, float* k, uint32_t 
                           uint32_t head_dim, uint32_t start_pos, const float* cos_t, const float* sin_t, uint32_t table_len);
 int launch_rope_paged_append(granite_cuda_compute* c, const GraniteCudaRopeAppendArgs& a);
 int launch_tree_commit(granite_cuda_compute* c, const GraniteCudaTreeCommitArgs& a);
-int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a);
-// What distinguishes an 8-bit or windowed attention call from the plain one: the cache's element type and scales (elem as
-// in q8.cuh: 0 fp16, 1 int8, 2 e4m3) and the window (0: none).
-struct CacheView {
-    int elem = 0;
-    const float* k_scales = nullptr;
-    const float* v_scales = nullptr;
-    uint32_t window = 0, sinks = 0;
-};
+int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a, const CacheView& view = CacheView{});
+int launch_paged_prefill_q8(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a, const CacheView& view);
 int launch_paged_decode_int8(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, const CacheView& view);
 int launch_paged_decode_e4m3(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, const CacheView& view);
 int launch_paged_decode_window(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint32_t max_seq, const CacheView& view);

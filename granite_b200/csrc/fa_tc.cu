@@ -36,10 +36,26 @@
 //               rescale of O).  With one tile per item O alternates between the two accumulators and
 //               a finished item is read out behind the next item's first MMAs.
 // TMEM (512 columns): S[0] | S[1] | O[0] | O[1], 128 fp32 columns each.
+//
+// Two views of the cache have builds of their own (prefill only):
+//
+//   kWindow   sliding window with sinks.  A query block walks the tiles of the sinks and then those from the window of its first
+//             row to its diagonal, so its work is that of the keys it can see; tiles at the edges are masked by column.  Pages
+//             that no row of the block sees are not looked up, and their V rows are cleared in shared memory like those
+//             past the live length.  A row may see nothing of a tile, or of all tiles (then it is zero).
+//   kQ8       codes of an 8-bit cache.  A small kernel first lays the chunk's pages out as fp16 codes (exact), contiguous
+//             per head, once for all query heads and blocks that read them - inside this kernel every block would convert
+//             them again, on the warps that are the pace setters already.  The scales stay fp32: with k and v the scales of a
+//             key's page, the weight 2^(s k scale - m) v / v_max is one exponential of a multiply-add, with (k scale) and
+//             log2(v / v_max) per page; the row sum adds a page's weights and multiplies by v_max / v once per page.  So the
+//             scales cost eight products per row and tile where the maxima are taken, and nothing per element.
+#include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "compute_internal.h"
 #include "ptx.cuh"
+#include "q8.cuh"
 
 namespace gb200 {
 
@@ -69,6 +85,13 @@ struct TcParams {
     const int32_t* cache_lens;  // [batch] or nullptr
     int batch, num_nodes, cache_len, cache_stride, max_blocks, num_blocks;
     int d_chunks;               // head_dim / 64: 2 (head_dim 128) or 1 (head_dim 64, half of every tile slot is used)
+    int window, sinks;          // kWindow; window 0: none
+    // kQ8: per (KV head, page), page_stride apart (a multiple of eight): k * scale_log2, log2(v / v_max), v_max / v; v_max per KV head
+    const float* page_k;
+    const float* page_lv;
+    const float* page_iv;
+    const float* v_max;
+    int page_stride;
     int slot_shift;             // tree: a tile is (128 >> slot_shift) query heads x (1 << slot_shift) node slots
 };
 
@@ -83,9 +106,18 @@ struct TcItem {
     int cache_len;  // tree: prefix length
     bool valid;
 };
+struct TcWindowItem : TcItem {
+    int n_sink;  // tiles of the sinks, walked first
+    int w0;      // first tile of the window
+    int lo;      // first key that any row's window holds; keys [sinks, lo) are hidden from all rows
+};
+// K/V tile of step j
+__device__ __forceinline__ int tile_of(const TcItem&, int j) { return j; }
+__device__ __forceinline__ int tile_of(const TcWindowItem& it, int j) { return j >= it.n_sink ? j - it.n_sink + it.w0 : j; }
 
 constexpr int kMaxCachedItems = 32;  // work items of a CTA kept in shared memory (later rounds are derived on the fly)
 
+template <typename Item>
 struct TcSmem {
     uint64_t q_full, q_empty, k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
     uint64_t s_full[2], s_free[2], p_ready[2];
@@ -95,9 +127,9 @@ struct TcSmem {
     uint64_t o_final[2];
     uint32_t tmem_base;
     int abort_flag;
-    TcItem items[kMaxCachedItems];  // item of round r, worked out once at start-up instead of by every role at every item boundary
+    Item items[kMaxCachedItems];  // item of round r, worked out once at start-up instead of by every role at every item boundary
 };
-static_assert(sizeof(TcSmem) <= 3072, "the barriers must fit beside seven 32 KB tiles");
+static_assert(sizeof(TcSmem<TcWindowItem>) <= 3072, "the barriers must fit beside seven 32 KB tiles");
 
 
 // fp32 -> fp16 hi + fp16 lo (x ~= hi + lo to about 22 bits), so fp32 queries lose nothing.
@@ -139,18 +171,21 @@ __global__ void tree_mask_kernel(const int32_t* parents, unsigned long long* mas
 // kTree:   tree verification (else causal prefill).   kPaged: tree prefix in the paged pool.
 // kSplitQ: queries given as fp16 hi + lo arrays (fp32 queries): S = Q_hi K^T + Q_lo K^T; one tile only.
 // kTiles:  query tiles per item (1 or 2).
-template <bool kTree, bool kPaged, bool kSplitQ, int kTiles>
+// kWindow, kQ8: see the top of the file.
+template <bool kTree, bool kPaged, bool kSplitQ, int kTiles, bool kWindow = false, bool kQ8 = false>
 __global__ void __launch_bounds__(kTcThreads, 1)
 fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap qlomap,
              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
              const __grid_constant__ CUtensorMap ktmap, const __grid_constant__ CUtensorMap vtmap, TcParams p) {
     static_assert(!(kSplitQ && kTiles == 2), "split queries take both query slots");
+    using Item = std::conditional_t<kWindow, TcWindowItem, TcItem>;
+    using Smem = TcSmem<Item>;
     constexpr int kQSlots = kSplitQ ? 2 : kTiles;
     constexpr int kStages = kQSlots == 1 ? 3 : 2;
     // barriers first, then the 1024-byte aligned tiles (128-byte swizzle atoms)
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    TcSmem* sh = reinterpret_cast<TcSmem*>(smem_raw);
-    uint8_t* q_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + sizeof(TcSmem) + 1023) & ~uintptr_t(1023));
+    Smem* sh = reinterpret_cast<Smem*>(smem_raw);
+    uint8_t* q_smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + sizeof(Smem) + 1023) & ~uintptr_t(1023));
     uint8_t* k_smem = q_smem + kQSlots * kTileBytes;
     uint8_t* v_smem = k_smem + kStages * kTileBytes;
     volatile int* abort_flag = &sh->abort_flag;
@@ -179,7 +214,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                               : p.n_qblocks * p.batch * p.num_kv_heads * p.units_per_kvh;
     const int n_rounds = (n_items + (int)gridDim.x - 1) / (int)gridDim.x;
     auto derive_item = [&](int r) {
-        TcItem it;
+        Item it;
         const int pos = r * (int)gridDim.x + ((r & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
         it.valid = pos < n_items;
         int pp = it.valid ? pos : 0;
@@ -210,6 +245,15 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             it.rows_here = min(kT, p.seq_q - it.q0);
             const int k_end = min(p.seq_kv, p.start_pos + it.q0 + it.rows_here);  // exclusive: last visible key + 1
             it.n_steps = (k_end + kT - 1) / kT;
+            if constexpr (kWindow) {
+                const int first_pos = p.start_pos + it.q0;
+                it.lo = window_span(first_pos, p.window, p.sinks).lo;
+                const int tiles = it.n_steps;
+                it.w0 = min(it.lo / kT, tiles);
+                it.n_sink = min((min(p.sinks, it.lo) + kT - 1) / kT, it.w0);
+                it.n_steps = max(it.n_sink + tiles - it.w0, 1);  // (a block that sees nothing still runs one, masked, step)
+                if (it.n_sink + tiles - it.w0 < 1) it.w0 = 0;
+            }
             it.n_prefix = it.n_steps;
             it.cache_len = p.seq_kv;  // paged K/V: pages past the live length are not looked up
         }
@@ -272,7 +316,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             uint32_t ph = 1;  // a fresh barrier passes a wait on parity 1
             int alive = 1;
             for (int r = 0; r < n_rounds && alive; r++) {
-                const TcItem it = item_of(r);
+                const Item it = item_of(r);
                 if (!it.valid) continue;
                 if (lane == 0) {
                     // the query tiles are replaced once the last score MMA of the previous item is done
@@ -305,8 +349,10 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 auto load_entry = [&](int j) {
                     int e = 0;
                     if (kPaged && j < it.n_prefix && lane < 8) {
-                        const int logical = j * 8 + lane;
-                        if (logical * kPageRows < it.cache_len) {
+                        const int logical = tile_of(it, j) * 8 + lane;
+                        bool hidden = false;  // from every row of the block
+                        if constexpr (kWindow) hidden = logical * kPageRows >= p.sinks && (logical + 1) * kPageRows <= it.lo;
+                        if (logical * kPageRows < it.cache_len && !hidden) {
                             e = p.tables[(size_t)it.b * p.max_blocks + logical];
                             if (e < 0 || e >= p.num_blocks) {
                                 atomicOr(p.status, kStatusBadTable);
@@ -358,7 +404,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         } else if (lane < p.d_chunks) {
                             // contiguous cache [.., max rows, 128]: one 128-row box per chunk
                             const int y = kTree ? (it.b * p.num_kv_heads + it.kvh) * p.cache_stride + j * kT
-                                                : (it.b * p.num_kv_heads + it.kvh) * p.max_seq + j * kT;
+                                                : (it.b * p.num_kv_heads + it.kvh) * p.max_seq + tile_of(it, j) * kT;
                             tma_load_2d(dst + c * kChunkBytes, is_v ? &vmap : &kmap, full, c * 64, y);
                         }
                     }
@@ -383,7 +429,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 int vs = 0;  // virtual steps issued so far across items: S buffer = vs & 1
                 uint32_t ph = 0;
                 for (int r = 0; r < n_rounds && ok; r++) {
-                    const TcItem it = item_of(r);
+                    const Item it = item_of(r);
                     if (!it.valid) continue;
                     ok = mbar_wait(&sh->q_full, items_done & 1, abort_flag);
                     items_done++;
@@ -446,7 +492,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 int st = 0, vs = 0, items_done = 0;
                 uint32_t ph = 0;
                 for (int r = 0; r < n_rounds && ok; r++) {
-                    const TcItem it = item_of(r);
+                    const Item it = item_of(r);
                     if (!it.valid) continue;
                     // one tile per item: O alternates between the two accumulators from item to item,
                     // so the previous item's result can be read out while this one accumulates
@@ -565,15 +611,17 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         };
 
         for (int r = 0; r < n_rounds; r++) {
-            const TcItem it = item_of(r);
+            const Item it = item_of(r);
             if (!it.valid) continue;
             // prefill: the last key a row may see; tree: the row's ancestor word, pre-shifted to this
             // thread's first column
             int last_visible[2];
+            int first_visible[2];  // kWindow: first key of the row's window
             unsigned long long anc[2] = {1ull >> (2 * tq), 1ull >> (2 * tq)};  // rows past the last node see column 0 only
 #pragma unroll
             for (int q = 0; q < 2; q++) {
                 last_visible[q] = kTree ? it.cache_len - 1 : min(p.start_pos + it.q0 + row_of[q], p.seq_kv - 1);
+                if (kWindow) first_visible[q] = window_span(p.start_pos + it.q0 + row_of[q], p.window, p.sinks).lo;
                 const int node = row_of[q] & ((1 << p.slot_shift) - 1);
                 if (kTree && node < N) {
                     const int32_t* par = p.parents + (size_t)it.b * N;
@@ -603,10 +651,24 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             }
             for (int j = 0; j < it.n_steps; j++, kvs++) {
                 const bool tree_step = kTree && j == it.n_prefix;
-                const int k0 = j * kT;
+                const int k0 = tile_of(it, j) * kT;
                 // prefill: the diagonal tile and a ragged last tile; tree prefix: a ragged last tile
+                // a window: and tiles that reach below the last row's window without being all sinks
                 const bool need_mask = kTree ? (!tree_step && k0 + kT > it.cache_len)
-                                             : ((k0 + kT - 1 > p.start_pos + it.q0) || (k0 + kT > p.seq_kv));
+                                             : ((k0 + kT - 1 > p.start_pos + it.q0) || (k0 + kT > p.seq_kv) ||
+                                                (kWindow && p.window > 0 && k0 < p.start_pos + it.q0 + kT - p.window && k0 + kT > p.sinks));
+                float page_k[kQ8 ? 8 : 1], page_lv[kQ8 ? 8 : 1];
+                const float* page_iv = nullptr;
+                if constexpr (kQ8) {
+                    const size_t at = (size_t)it.kvh * p.page_stride + (size_t)(k0 / kPageRows);
+                    page_iv = p.page_iv + at;
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const float4 a = __ldg(reinterpret_cast<const float4*>(p.page_k + at) + c), b = __ldg(reinterpret_cast<const float4*>(p.page_lv + at) + c);
+                        page_k[4 * c] = a.x; page_k[4 * c + 1] = a.y; page_k[4 * c + 2] = a.z; page_k[4 * c + 3] = a.w;
+                        page_lv[4 * c] = b.x; page_lv[4 * c + 1] = b.y; page_lv[4 * c + 2] = b.z; page_lv[4 * c + 3] = b.w;
+                    }
+                }
                 // not unrolled: the two tiles of an item share one copy of the softmax code
 #pragma unroll 1
                 for (int t = 0; t < kTiles; t++, vs++) {
@@ -640,13 +702,17 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 #pragma unroll
                         for (int q = 0; q < 2; q++) {
                             const int limit = last_visible[q] - k0 - 2 * tq;  // own column 64 h + 8 i + e is visible iff <= limit
+                            // ... and, with a window, >= low or < sink
+                            const int low = kWindow ? first_visible[q] - k0 - 2 * tq : 0, sink = kWindow ? min(p.sinks, first_visible[q]) - k0 - 2 * tq : 0;
 #pragma unroll
                             for (int h = 0; h < 2; h++)
 #pragma unroll
                                 for (int i = 0; i < 8; i++)
 #pragma unroll
-                                    for (int e = 0; e < 2; e++)
-                                        if (64 * h + 8 * i + e > limit) x[h][4 * i + 2 * q + e] = kNegInf;
+                                    for (int e = 0; e < 2; e++) {
+                                        const int col = 64 * h + 8 * i + e;
+                                        if (col > limit || (kWindow && col < low && col >= sink)) x[h][4 * i + 2 * q + e] = kNegInf;
+                                    }
                         }
                     }
                     float mx[2];
@@ -656,12 +722,23 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 #pragma unroll
                         for (int h = 0; h < 2; h++)
 #pragma unroll
-                            for (int i = 0; i < 8; i++)
-                                mm[h] = max3(mm[h], __uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1]));
+                            for (int i = 0; i < 8; i++) {
+                                if constexpr (kQ8) {
+                                    // a page is two of the thread's column pairs; its scale is positive
+                                    if (i & 1) continue;
+                                    const float pm = fmaxf(max3(__uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1]),
+                                                                __uint_as_float(x[h][4 * i + 4 + 2 * q])),
+                                                           __uint_as_float(x[h][4 * i + 4 + 2 * q + 1]));
+                                    mm[h] = fmaxf(mm[h], pm * page_k[4 * h + i / 2]);
+                                } else {
+                                    mm[h] = max3(mm[h], __uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1]));
+                                }
+                            }
                         float m = fmaxf(mm[0], mm[1]);
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                        mx[q] = m * p.scale_log2;
+                        mx[q] = kQ8 ? m : m * p.scale_log2;
+                        if (kWindow) mx[q] = fmaxf(mx[q], -1e30f);  // a row that sees nothing of the tile: finite, so that -inf scores give weight 0
                     }
                     if (j == 0) {
                         m_used[0] = mx[0];
@@ -705,6 +782,29 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         for (int h = 0; h < 2; h++) {
                             if (tree_step && h == 1) continue;
                             uint32_t hi[16], lo[16];
+            if constexpr (kQ8) {
+#pragma unroll
+                            for (int pg = 0; pg < 4; pg++) {
+                                const float iv = __ldg(page_iv + 4 * h + pg);
+                                const uint64_t iv2 = f32x2(iv, iv), k2 = f32x2(page_k[4 * h + pg], page_k[4 * h + pg]);
+#pragma unroll
+                                for (int q = 0; q < 2; q++) {
+                                    // 2^(s k - m + log2(v / v_max)); masked scores are -inf and give exactly 0
+                                    const float off = page_lv[4 * h + pg] - m_used[q];
+                                    const uint64_t off2 = f32x2(off, off);
+                                    uint64_t pair[2];
+#pragma unroll
+                                    for (int i2 = 0; i2 < 2; i2++) {
+                                        const int i = 2 * pg + i2;
+                                        float t0, t1;
+                                        f32x2_get(fma_f32x2(f32x2(__uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1])), k2, off2), t0, t1);
+                                        pair[i2] = f32x2(fast_exp2(t0), fast_exp2(t1));
+                                        split_hi_lo_x2(pair[i2], hi[2 * i + q], lo[2 * i + q]);
+                                    }
+                                    ls[q][pg & 1] = fma_f32x2(add_f32x2(pair[0], pair[1]), iv2, ls[q][pg & 1]);
+                                }
+                            }
+            } else {
 #pragma unroll
                             for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -717,6 +817,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                                     ls[q][i & 1] = add_f32x2(ls[q][i & 1], pp);
                                     split_hi_lo_x2(pp, hi[2 * i + q], lo[2 * i + q]);
                                 }
+            }
                             tmem_st_16x128b_x8(s_frag + 32 * h, hi);
                             tmem_st_16x128b_x8(s_frag + 64 + 32 * h, lo);
                         }
@@ -727,18 +828,30 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                             l_run[q] += la + lb;
                         }
                     }
-                    if (t == 0 && wg == 0 && need_mask && k0 + kT > (kTree ? it.cache_len : p.seq_kv)) {
-                        // keys past the live length carry P = 0, but their V rows may hold anything (even
-                        // NaN): zero them in shared memory before the MMAs read the tile
+                    bool clear_v = k0 + kT > (kTree ? it.cache_len : p.seq_kv);
+                    if constexpr (kWindow) clear_v |= k0 + kT > p.sinks && k0 < it.lo;
+                    if (t == 0 && wg == 0 && need_mask && clear_v) {
+                        // keys past the live length (and those that the window hides from every row) carry P = 0, but their V
+                        // rows may hold anything (even NaN): zero them in shared memory before the MMAs read the tile
                         const int st = kvs % kStages;
                         ok = __all_sync(0xffffffffu, ok && mbar_wait(&sh->v_full[st], (kvs / kStages) & 1, abort_flag));
-                        const int first_bad = (kTree ? it.cache_len : p.seq_kv) - k0;
                         uint8_t* vt = v_smem + st * kTileBytes;
                         const int row_units = 8 * p.d_chunks;  // 16-byte units per V row
-                        for (int i = row; i < (kT - first_bad) * row_units; i += 128) {
-                            const int vr = first_bad + i / row_units, u = i % row_units;
-                            *reinterpret_cast<uint4*>(vt + (vr >> 3) * group_bytes + (u >> 3) * chunk_off + (vr & 7) * 128 +
-                                                      (((u & 7) ^ (vr & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                        // rows [lo, hi) of the tile that only a window hides; then those past the live length
+                        int lo = 0, hi = 0;
+                        if constexpr (kWindow) {
+                            lo = min(max(p.sinks - k0, 0), kT);
+                            hi = min(max(it.lo - k0, 0), kT);
+                        }
+#pragma unroll
+                        for (int part = kWindow ? 0 : 1; part < 2; part++) {
+                            const int first_bad = part ? (kWindow ? min(max(p.seq_kv - k0, 0), kT) : (kTree ? it.cache_len : p.seq_kv) - k0) : lo;
+                            const int end = part ? kT : hi;
+                            for (int i = row; i < (end - first_bad) * row_units; i += 128) {
+                                const int vr = first_bad + i / row_units, u = i % row_units;
+                                *reinterpret_cast<uint4*>(vt + (vr >> 3) * group_bytes + (u >> 3) * chunk_off + (vr & 7) * 128 +
+                                                          (((u & 7) ^ (vr & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                            }
                         }
                         fence_proxy_async_smem();
                     }
@@ -769,6 +882,8 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     l += __shfl_xor_sync(0xffffffffu, l, 1);
                     l += __shfl_xor_sync(0xffffffffu, l, 2);
                     e.inv[q] = __frcp_rn(l);
+                    if (kWindow && !(l > 0.f)) e.inv[q] = 0.f;  // a row that sees nothing
+                    if (kQ8) e.inv[q] *= p.v_max[it.kvh];
                     if (kTree) {
                         const int node = row_of[q] & ((1 << p.slot_shift) - 1);
                         const int head = it.head0 + (kT >> p.slot_shift) * t + (row_of[q] >> p.slot_shift);
@@ -808,7 +923,7 @@ static int launch_tc(granite_cuda_compute* c, TcKernel kern, const char* name, i
                      const CUtensorMap* vmap, const CUtensorMap* ktmap, const CUtensorMap* vtmap, const TcParams& p) {
     // Q slots + K and V rings: 3 stages fit beside one query slot, 2 beside two
     const int stages = q_slots == 1 ? 3 : 2;
-    size_t smem_bytes = (sizeof(TcSmem) + 1023) / 1024 * 1024 + 1024 + (size_t)(q_slots + 2 * stages) * kTileBytes;
+    size_t smem_bytes = (sizeof(TcSmem<TcWindowItem>) + 1023) / 1024 * 1024 + 1024 + (size_t)(q_slots + 2 * stages) * kTileBytes;
     if (smem_bytes > (size_t)c->smem_optin) smem_bytes = (size_t)c->smem_optin;  // the window is 1 KB aligned in practice
     GB_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes));
     const int grid = n_items < c->sm_count ? n_items : c->sm_count;  // persistent CTAs, one per SM
@@ -820,10 +935,16 @@ static int launch_tc(granite_cuda_compute* c, TcKernel kern, const char* name, i
     return GRANITE_CUDA_SUCCESS;
 }
 
-// fp32 queries -> hi / lo fp16 arrays in the scratch arena
-static int split_queries(granite_cuda_compute* c, const void* q, size_t n, const void** hi_out, const void** lo_out) {
-    const size_t half_bytes = (n * 2 + 255) / 256 * 256;
-    int rc = c->ensure_scratch(2 * half_bytes);
+static void set_window(TcParams& p, const CacheView& view) {
+    p.window = (int)std::min(view.window, 0x7fffffffu);
+    p.sinks = (int)std::min(view.sinks, 0x7fffffffu);
+}
+
+// fp32 queries -> hi / lo fp16 arrays at the start of the scratch arena, which is made large enough for `behind` bytes after them
+static size_t split_bytes(size_t n) { return 2 * ((n * 2 + 255) / 256 * 256); }
+static int split_queries(granite_cuda_compute* c, const void* q, size_t n, const void** hi_out, const void** lo_out, size_t behind = 0) {
+    const size_t half_bytes = split_bytes(n) / 2;
+    int rc = c->ensure_scratch(2 * half_bytes + behind);
     if (rc) return rc;
     LaunchScope t(c, "split_q_f16");
     __half* hi = static_cast<__half*>(c->scratch);
@@ -834,9 +955,9 @@ static int split_queries(granite_cuda_compute* c, const void* q, size_t n, const
     return GRANITE_CUDA_SUCCESS;
 }
 
-int launch_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a) {
+int launch_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, const CacheView& view) {
     if (!a.q || !a.k || !a.v || !a.output) return fail(GRANITE_CUDA_NULL_POINTER, "prefill: null buffer");
-    if (a.head_dim != 128 && a.head_dim != 64) return launch_generic_prefill(c, a);  // the plain kernel takes the other head dims
+    if (a.head_dim != 128 && a.head_dim != 64) return launch_generic_prefill(c, a, view);  // the plain kernel takes the other head dims
     const uint32_t D = a.head_dim;
     if (a.num_kv_heads == 0 || a.num_heads % a.num_kv_heads != 0)
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, "prefill: num_heads must be a multiple of num_kv_heads");
@@ -881,16 +1002,20 @@ int launch_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a) {
     if (!qmap || !qlomap || !kmap || !vmap) return GRANITE_CUDA_EXECUTION_FAILED;
 
     TcKernel kern = split_q ? fa_tc_kernel<false, false, true, 1> : fa_tc_kernel<false, false, false, 1>;
+    if (view.window > 0) {
+        set_window(p, view);
+        kern = split_q ? fa_tc_kernel<false, false, true, 1, true> : fa_tc_kernel<false, false, false, 1, true>;
+    }
     const int n_items = p.n_qblocks * p.batch * p.num_kv_heads * p.units_per_kvh;
-    return launch_tc(c, kern, "prefill_causal_fa", n_items, split_q ? 2 : tiles, qmap, qlomap, kmap, vmap, kmap, vmap, p);
+    return launch_tc(c, kern, view.window > 0 ? "prefill_window_fa" : "prefill_causal_fa", n_items, split_q ? 2 : tiles, qmap, qlomap, kmap, vmap, kmap, vmap, p);
 }
 
 // Causal attention of a chunk of new tokens against the sequence's paged cache: the prefill
 // kernel with its K/V tiles gathered page by page through the block table.
-int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a) {
+int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a, const CacheView& view) {
     if (!a.q || !a.k_cache || !a.v_cache || !a.block_table || !a.output)
         return fail(GRANITE_CUDA_NULL_POINTER, "paged_prefill_attention: null buffer");
-    if ((a.head_dim != 128 && a.head_dim != 64) || a.block_size != (uint32_t)kPageRows) return launch_generic_paged_prefill(c, a);
+    if ((a.head_dim != 128 && a.head_dim != 64) || a.block_size != (uint32_t)kPageRows) return launch_generic_paged_prefill(c, a, view);
     const uint32_t D = a.head_dim;
     if (a.num_blocks == 0 || a.max_blocks_per_seq == 0)
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, "paged_prefill_attention: empty pool or table");
@@ -937,8 +1062,189 @@ int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillA
     if (!qmap || !qlomap || !kmap || !vmap) return GRANITE_CUDA_EXECUTION_FAILED;
 
     TcKernel kern = split_q ? fa_tc_kernel<false, true, true, 1> : fa_tc_kernel<false, true, false, 1>;
+    if (view.window > 0) {
+        set_window(p, view);
+        kern = split_q ? fa_tc_kernel<false, true, true, 1, true> : fa_tc_kernel<false, true, false, 1, true>;
+    }
     const int n_items = p.n_qblocks * p.num_kv_heads * p.units_per_kvh;
-    return launch_tc(c, kern, "paged_prefill_fa", n_items, split_q ? 2 : 1, qmap, qlomap, kmap, vmap, kmap, vmap, p);
+    return launch_tc(c, kern, view.window > 0 ? "paged_prefill_window_fa" : "paged_prefill_fa", n_items, split_q ? 2 : 1, qmap, qlomap, kmap, vmap, kmap, vmap, p);
+}
+
+// ------------------------------------------------------------------------------------ 8-bit cache
+struct Q8GatherParams {
+    const uint8_t* k;      // pools [num_blocks * 16, Hkv, D]
+    const uint8_t* v;
+    const float* k_scales;
+    const float* v_scales;
+    const int32_t* table;
+    __half* k16;           // [Hkv, rows, D]
+    __half* v16;
+    float* page_k;         // see TcParams
+    float* page_lv;
+    float* page_iv;
+    float* v_max;
+    int hkv, d, rows, n_pages, page_stride, num_blocks;
+    int head_pages, skip;  // visible pages: entry i is page i before head_pages, i + skip from there on; n_pages - skip of them
+    float scale_log2;
+    int* status;
+};
+
+// One launch in front of the attention kernel.  Blocks [0, Hkv): the page scales of one KV head in the form the softmax wants
+// them.  The others: a page's codes to fp16, one block per page, 16 codes of K and of V per thread at a time - a page is read
+// and written in whole rows, three bytes of traffic per code.
+template <int kElem>
+__global__ void __launch_bounds__(256) q8_gather_kernel(const __grid_constant__ Q8GatherParams p) {
+    const int tid = threadIdx.x;
+    const int visible = p.n_pages - p.skip;
+    auto page_of = [&](int i) { return i < p.head_pages ? i : i + p.skip; };
+    auto entry_of = [&](int page) {
+        const int e = p.table[page];
+        return e < 0 || e >= p.num_blocks ? -1 : e;
+    };
+    if ((int)blockIdx.x < p.hkv) {
+        const int h = blockIdx.x;
+        __shared__ float s_red[8];
+        float m = 0.f;
+        for (int i = tid; i < visible; i += 256) {
+            const int e = entry_of(page_of(i));
+            if (e >= 0) m = fmaxf(m, p.v_scales[(size_t)e * p.hkv + h]);
+        }
+#pragma unroll
+        for (int sh = 16; sh > 0; sh >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
+        if ((tid & 31) == 0) s_red[tid >> 5] = m;
+        __syncthreads();
+        for (int w = 0; w < 8; w++) m = fmaxf(m, s_red[w]);
+        if (!(m > 0.f)) m = 1.f;  // every V code is zero
+        if (tid == 0) p.v_max[h] = m;
+        for (int page = tid; page < p.page_stride; page += 256) {
+            // pages of a visible tile that are not visible themselves: any finite numbers (their scores are masked)
+            float k = 1.f, v = m;
+            if (page < p.n_pages && (page < p.head_pages || page >= p.head_pages + p.skip)) {
+                const int e = entry_of(page);
+                if (e >= 0) {
+                    k = p.k_scales[(size_t)e * p.hkv + h];
+                    v = p.v_scales[(size_t)e * p.hkv + h];
+                }
+            }
+            // scale 0 comes with zero codes, so any positive number stands for it; 2^-60 of the largest V scale is beyond fp32 sums
+            k = fmaxf(k, 1e-30f);
+            const float r = fmaxf(__fdiv_rn(v, m), 8.67361738e-19f);
+            const size_t at = (size_t)h * p.page_stride + page;
+            p.page_k[at] = k * p.scale_log2;
+            p.page_lv[at] = log2f(r);
+            p.page_iv[at] = __fdiv_rn(1.f, r);
+        }
+        return;
+    }
+    const int page = page_of(blockIdx.x - p.hkv);
+    const int e = entry_of(page);
+    if (e < 0 && tid == 0) atomicOr(p.status, kStatusBadTable);
+    const int row_units = p.hkv * p.d / 16, head_units = p.d / 16;  // 16-code units
+    const uint4 *k = reinterpret_cast<const uint4*>(p.k) + (size_t)(e < 0 ? 0 : e) * kPageRows * row_units;
+    const uint4 *v = reinterpret_cast<const uint4*>(p.v) + (size_t)(e < 0 ? 0 : e) * kPageRows * row_units;
+    for (int i = tid; i < kPageRows * row_units; i += 256) {
+        // consecutive threads: the units of a head's row, then the rows of that head (the destination's order)
+        const int u = i % head_units, r = (i / head_units) % kPageRows, h = i / (head_units * kPageRows);
+        const int src = r * row_units + h * head_units + u;
+        const uint4 kc = e < 0 ? make_uint4(0, 0, 0, 0) : k[src], vc = e < 0 ? make_uint4(0, 0, 0, 0) : v[src];
+        const size_t dst = (((size_t)h * p.rows + (size_t)page * kPageRows + r) * p.d + u * 16) / 8;
+        auto store = [&](uint4* out, const uint4& c) {
+            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+            uint32_t y[8];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const float4 f = q8_decode4<kElem>(w[q]);
+                y[2 * q] = pack_half2(f.x, f.y);
+                y[2 * q + 1] = pack_half2(f.z, f.w);
+            }
+            out[0] = make_uint4(y[0], y[1], y[2], y[3]);
+            out[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        };
+        store(reinterpret_cast<uint4*>(p.k16) + dst, kc);
+        store(reinterpret_cast<uint4*>(p.v16) + dst, vc);
+    }
+}
+
+// Chunked prefill over the 8-bit cache: the chunk's visible pages become fp16 codes in the scratch arena, then the
+// attention kernel runs over them as over a contiguous cache, with the pages' scales beside it.
+int launch_paged_prefill_q8(granite_cuda_compute* c, const GraniteCudaPagedPrefillArgs& a, const CacheView& view) {
+    if ((a.head_dim != 128 && a.head_dim != 64) || a.block_size != (uint32_t)kPageRows) return launch_generic_paged_prefill(c, a, view);
+    const uint32_t D = a.head_dim;
+    const bool split_q = a.q_dtype == 0;
+    TcParams p{};
+    set_window(p, view);
+    p.d_chunks = (int)D / 64;
+    p.num_heads = (int)a.num_heads;
+    p.num_kv_heads = (int)a.num_kv_heads;
+    p.group = (int)(a.num_heads / a.num_kv_heads);
+    p.units_per_kvh = p.group;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.status = c->d_status;
+    p.out = a.output;
+    p.out_fp16 = a.out_dtype == 1;
+    p.seq_q = (int)a.seq_q;
+    p.seq_kv = (int)(a.start_pos + a.seq_q);
+    p.n_qblocks = (p.seq_q + kT - 1) / kT;
+    p.start_pos = (int)a.start_pos;
+    p.batch = 1;
+
+    Q8GatherParams g{};
+    g.hkv = p.num_kv_heads;
+    g.d = (int)D;
+    g.n_pages = (p.seq_kv + kPageRows - 1) / kPageRows;
+    g.page_stride = (g.n_pages + 7) / 8 * 8;
+    g.rows = g.page_stride * kPageRows;
+    p.max_seq = g.rows;
+    p.page_stride = g.page_stride;
+    if ((uint64_t)g.hkv * g.rows >= (1ull << 31) || (uint64_t)p.n_qblocks * a.num_heads >= (1ull << 31))
+        return fail(GRANITE_CUDA_INVALID_ARGUMENT, "paged_prefill_attention_q8: num_kv_heads * length exceeds the tensor-map coordinate range");
+    {
+        const WindowSpan w = window_span(p.start_pos, p.window, p.sinks);
+        const int first = w.lo / kPageRows;
+        g.head_pages = std::min((w.sinks_end + kPageRows - 1) / kPageRows, first);
+        g.skip = first - g.head_pages;
+    }
+    const size_t n_q = (size_t)a.seq_q * a.num_heads * D;
+    const size_t q_bytes = split_q ? split_bytes(n_q) : 0;
+    const size_t kv_bytes = (size_t)g.hkv * g.rows * D * 2;                                           // a multiple of 128 rows * 128 bytes
+    const size_t page_bytes = ((size_t)g.hkv * g.page_stride * 4 + 255) / 256 * 256;
+    const size_t behind = 2 * kv_bytes + 3 * page_bytes + ((size_t)g.hkv * 4 + 255) / 256 * 256;
+    const void *q16 = a.q, *q16_lo = a.q;
+    int rc = split_q ? split_queries(c, a.q, n_q, &q16, &q16_lo, behind) : c->ensure_scratch(behind);
+    if (rc) return rc;
+    uint8_t* ws = static_cast<uint8_t*>(c->scratch) + q_bytes;
+    g.k16 = reinterpret_cast<__half*>(ws);
+    g.v16 = reinterpret_cast<__half*>(ws + kv_bytes);
+    g.page_k = reinterpret_cast<float*>(ws + 2 * kv_bytes);
+    g.page_lv = reinterpret_cast<float*>(ws + 2 * kv_bytes + page_bytes);
+    g.page_iv = reinterpret_cast<float*>(ws + 2 * kv_bytes + 2 * page_bytes);
+    g.v_max = reinterpret_cast<float*>(ws + 2 * kv_bytes + 3 * page_bytes);
+    g.k = static_cast<const uint8_t*>(a.k_cache);
+    g.v = static_cast<const uint8_t*>(a.v_cache);
+    g.k_scales = view.k_scales;
+    g.v_scales = view.v_scales;
+    g.table = a.block_table;
+    g.num_blocks = (int)a.num_blocks;
+    g.scale_log2 = p.scale_log2;
+    g.status = c->d_status;
+    {
+        LaunchScope t(c, "q8_gather_f16");
+        auto kern = view.elem == kElemInt8 ? q8_gather_kernel<kElemInt8> : q8_gather_kernel<kElemE4M3>;
+        kern<<<(unsigned)(g.hkv + g.n_pages - g.skip), 256, 0, c->stream>>>(g);
+        GB_CUDA_TRY(cudaGetLastError());
+    }
+    p.page_k = g.page_k;
+    p.page_lv = g.page_lv;
+    p.page_iv = g.page_iv;
+    p.v_max = g.v_max;
+    const CUtensorMap* qmap = c->tensor_map_2d(q16, (uint64_t)a.num_heads * D, a.seq_q, (uint64_t)a.num_heads * D * 2, 64, kT, 128);
+    const CUtensorMap* qlomap = c->tensor_map_2d(q16_lo, (uint64_t)a.num_heads * D, a.seq_q, (uint64_t)a.num_heads * D * 2, 64, kT, 128);
+    const CUtensorMap* kmap = c->tensor_map_2d(g.k16, D, (uint64_t)g.hkv * g.rows, D * 2, 64, kT, 128);
+    const CUtensorMap* vmap = c->tensor_map_2d(g.v16, D, (uint64_t)g.hkv * g.rows, D * 2, 64, kT, 128);
+    if (!qmap || !qlomap || !kmap || !vmap) return GRANITE_CUDA_EXECUTION_FAILED;
+    TcKernel kern = split_q ? fa_tc_kernel<false, false, true, 1, true, true> : fa_tc_kernel<false, false, false, 1, true, true>;
+    const int n_items = p.n_qblocks * p.num_kv_heads * p.units_per_kvh;
+    return launch_tc(c, kern, "paged_prefill_q8_fa", n_items, split_q ? 2 : 1, qmap, qlomap, kmap, vmap, kmap, vmap, p);
 }
 
 int launch_tree_mask(granite_cuda_compute* c, const int32_t* parents, uint64_t* masks, uint32_t batch, uint32_t n) {
