@@ -133,15 +133,32 @@ static_assert(sizeof(TcSmem<TcWindowItem>) <= 3072, "the barriers must fit besid
 
 
 // fp32 -> fp16 hi + fp16 lo (x ~= hi + lo to about 22 bits), so fp32 queries lose nothing.
-__global__ void split_f32_to_f16_kernel(const float* __restrict__ src, __half* __restrict__ hi,
-                                        __half* __restrict__ lo, size_t n) {
-    size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i < n) {
-        const float x = src[i];
-        const __half h = __float2half_rn(x);
-        hi[i] = h;
-        lo[i] = __float2half_rn(x - __half2float(h));
+// Eight values per thread, 16-byte accesses (n is a multiple of 64: whole heads): a 4001 x 32 x 128 chunk takes 22 us against 58
+// one value at a time.
+__global__ void split_f32_to_f16_kernel(const float4* __restrict__ src, uint4* __restrict__ hi, uint4* __restrict__ lo, size_t n8) {
+    const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n8) return;
+    const float4 a = src[2 * i], b = src[2 * i + 1];
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        h[k] = pack_half2(x[2 * k], x[2 * k + 1]);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+        l[k] = pack_half2(x[2 * k] - back.x, x[2 * k + 1] - back.y);
     }
+    hi[i] = make_uint4(h[0], h[1], h[2], h[3]);
+    lo[i] = make_uint4(l[0], l[1], l[2], l[3]);
+}
+// The same for a source that is not 16-byte aligned.
+__global__ void split_f32_to_f16_single_kernel(const float* __restrict__ src, __half* __restrict__ hi,
+                                               __half* __restrict__ lo, size_t n) {
+    const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= n) return;
+    const float x = src[i];
+    const __half h = __float2half_rn(x);
+    hi[i] = h;
+    lo[i] = __float2half_rn(x - __half2float(h));
 }
 
 // Ancestor word of one node: bit j set when the node may attend to tree node j (itself or an
@@ -949,7 +966,11 @@ static int split_queries(granite_cuda_compute* c, const void* q, size_t n, const
     LaunchScope t(c, "split_q_f16");
     __half* hi = static_cast<__half*>(c->scratch);
     __half* lo = reinterpret_cast<__half*>(static_cast<uint8_t*>(c->scratch) + half_bytes);
-    split_f32_to_f16_kernel<<<(unsigned)((n + 255) / 256), 256, 0, c->stream>>>(static_cast<const float*>(q), hi, lo, n);
+    if ((reinterpret_cast<uintptr_t>(q) & 15) == 0 && n % 8 == 0)
+        split_f32_to_f16_kernel<<<(unsigned)((n / 8 + 255) / 256), 256, 0, c->stream>>>(
+            static_cast<const float4*>(q), reinterpret_cast<uint4*>(hi), reinterpret_cast<uint4*>(lo), n / 8);
+    else
+        split_f32_to_f16_single_kernel<<<(unsigned)((n + 255) / 256), 256, 0, c->stream>>>(static_cast<const float*>(q), hi, lo, n);
     *hi_out = hi;
     *lo_out = lo;
     return GRANITE_CUDA_SUCCESS;
@@ -1142,26 +1163,40 @@ __global__ void __launch_bounds__(256) q8_gather_kernel(const __grid_constant__ 
     const int row_units = p.hkv * p.d / 16, head_units = p.d / 16;  // 16-code units
     const uint4 *k = reinterpret_cast<const uint4*>(p.k) + (size_t)(e < 0 ? 0 : e) * kPageRows * row_units;
     const uint4 *v = reinterpret_cast<const uint4*>(p.v) + (size_t)(e < 0 ? 0 : e) * kPageRows * row_units;
-    for (int i = tid; i < kPageRows * row_units; i += 256) {
-        // consecutive threads: the units of a head's row, then the rows of that head (the destination's order)
-        const int u = i % head_units, r = (i / head_units) % kPageRows, h = i / (head_units * kPageRows);
-        const int src = r * row_units + h * head_units + u;
-        const uint4 kc = e < 0 ? make_uint4(0, 0, 0, 0) : k[src], vc = e < 0 ? make_uint4(0, 0, 0, 0) : v[src];
-        const size_t dst = (((size_t)h * p.rows + (size_t)page * kPageRows + r) * p.d + u * 16) / 8;
-        auto store = [&](uint4* out, const uint4& c) {
-            const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-            uint32_t y[8];
+    auto widen = [&](uint4* out, const uint4& c) {
+        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        uint32_t y[8];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const float4 f = q8_decode4<kElem>(w[q]);
-                y[2 * q] = pack_half2(f.x, f.y);
-                y[2 * q + 1] = pack_half2(f.z, f.w);
+        for (int q = 0; q < 4; q++) {
+            const float4 f = q8_decode4<kElem>(w[q]);
+            y[2 * q] = pack_half2(f.x, f.y);
+            y[2 * q + 1] = pack_half2(f.z, f.w);
+        }
+        out[0] = make_uint4(y[0], y[1], y[2], y[3]);
+        out[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    };
+    constexpr int kUnits = 4;  // units of K and of V in flight per thread
+    const int n = kPageRows * row_units;
+    for (int base = tid; base < n; base += 256 * kUnits) {
+        uint4 kc[kUnits], vc[kUnits];
+#pragma unroll
+        for (int q = 0; q < kUnits; q++) {
+            // consecutive threads: the units of a head's row, then the rows of that head (the destination's order)
+            const int i = base + 256 * q, u = i % head_units, r = (i / head_units) % kPageRows, h = i / (head_units * kPageRows);
+            kc[q] = vc[q] = make_uint4(0, 0, 0, 0);
+            if (i < n && e >= 0) {
+                kc[q] = k[r * row_units + h * head_units + u];
+                vc[q] = v[r * row_units + h * head_units + u];
             }
-            out[0] = make_uint4(y[0], y[1], y[2], y[3]);
-            out[1] = make_uint4(y[4], y[5], y[6], y[7]);
-        };
-        store(reinterpret_cast<uint4*>(p.k16) + dst, kc);
-        store(reinterpret_cast<uint4*>(p.v16) + dst, vc);
+        }
+#pragma unroll
+        for (int q = 0; q < kUnits; q++) {
+            const int i = base + 256 * q, u = i % head_units, r = (i / head_units) % kPageRows, h = i / (head_units * kPageRows);
+            if (i >= n) break;
+            const size_t dst = (((size_t)h * p.rows + (size_t)page * kPageRows + r) * p.d + u * 16) / 8;
+            widen(reinterpret_cast<uint4*>(p.k16) + dst, kc[q]);
+            widen(reinterpret_cast<uint4*>(p.v16) + dst, vc[q]);
+        }
     }
 }
 

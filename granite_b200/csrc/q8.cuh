@@ -28,12 +28,13 @@ __device__ __forceinline__ float4 q8_decode4(uint32_t w) {
     return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// Round to nearest even into the code range.
+// Round to nearest even; |x| is at most the code range's end, up to a rounding error.
 template <int kElem>
 __device__ __forceinline__ uint32_t q8_encode4(float4 x) {
     if (kElem == kElemInt8) {
-        auto one = [](float f) { return (uint32_t)(min(max(__float2int_rn(f), -127), 127) & 0xFF); };
-        return one(x.x) | (one(x.y) << 8) | (one(x.z) << 16) | (one(x.w) << 24);
+        // adding 1.5 * 2^23 leaves the rounded integer in the low bits of the sum
+        auto one = [](float f) { return __float_as_uint(__fadd_rn(f, 12582912.f)); };
+        return __byte_perm(__byte_perm(one(x.x), one(x.y), 0x0040), __byte_perm(one(x.z), one(x.w), 0x0040), 0x5410);
     }
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x.x, x.y), __NV_SATFINITE, __NV_E4M3) |
            ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x.z, x.w), __NV_SATFINITE, __NV_E4M3) << 16);
