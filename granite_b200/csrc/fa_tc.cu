@@ -37,7 +37,10 @@
 //               a finished item is read out behind the next item's first MMAs.
 // TMEM (512 columns): S[0] | S[1] | O[0] | O[1], 128 fp32 columns each.
 //
-// Two views of the cache have builds of their own (prefill only):
+// Two views of the cache have builds of their own (prefill only).  Their items may also be cut along the keys (n_chunks):
+// each chunk leaves its un-normalised output, maximum and sum per row, and prefill_merge_kernel joins them.  That fills the SMs
+// when there are few query blocks, and it bounds the number of truncating additions in a tensor-core accumulator: one run
+// over 6144 keys was off by 1.2e-5 (growing with the length), 22 tiles by 7e-6.
 //
 //   kWindow   sliding window with sinks.  A query block walks the tiles of the sinks and then those from the window of its first
 //             row to its diagonal, so its work is that of the keys it can see; tiles at the edges are masked by column.  Pages
@@ -92,6 +95,10 @@ struct TcParams {
     const float* page_iv;
     const float* v_max;
     int page_stride;
+    // kWindow: pieces that every item's tiles are cut into; with more than one, [row, head, chunk] partials
+    int n_chunks;
+    float* part_o;
+    float2* part_ml;
     int slot_shift;             // tree: a tile is (128 >> slot_shift) query heads x (1 << slot_shift) node slots
 };
 
@@ -110,10 +117,36 @@ struct TcWindowItem : TcItem {
     int n_sink;  // tiles of the sinks, walked first
     int w0;      // first tile of the window
     int lo;      // first key that any row's window holds; keys [sinks, lo) are hidden from all rows
+    int j0;      // first of the item's steps in the query block's
+    int chunk;
 };
+// The steps of the query block that starts at row q0: tiles of the sinks, then from the window of its first row to its diagonal.
+struct WindowSteps {
+    int n, n_sink, w0, lo;
+};
+__host__ __device__ __forceinline__ WindowSteps window_steps(const TcParams& p, int q0) {
+    WindowSteps w;
+    const int rows = p.seq_q - q0 < kT ? p.seq_q - q0 : kT, last = p.start_pos + q0 + rows;
+    const int tiles = ((p.seq_kv < last ? p.seq_kv : last) + kT - 1) / kT;  // up to the last visible key
+    w.lo = window_span(p.start_pos + q0, p.window, p.sinks).lo;
+    w.w0 = w.lo / kT < tiles ? w.lo / kT : tiles;
+    const int sink_tiles = ((p.sinks < w.lo ? p.sinks : w.lo) + kT - 1) / kT;
+    w.n_sink = sink_tiles < w.w0 ? sink_tiles : w.w0;
+    w.n = w.n_sink + tiles - w.w0;
+    if (w.n < 1) {  // a block that sees nothing still runs one, masked, step
+        w.n = 1;
+        w.w0 = 0;
+    }
+    return w;
+}
+// Steps [chunk_begin(n, c), chunk_begin(n, c + 1)) of n are chunk c's; there are more chunks than steps in short blocks.
+__host__ __device__ __forceinline__ int chunk_begin(int n, int n_chunks, int c) { return n * c / n_chunks; }
 // K/V tile of step j
 __device__ __forceinline__ int tile_of(const TcItem&, int j) { return j; }
-__device__ __forceinline__ int tile_of(const TcWindowItem& it, int j) { return j >= it.n_sink ? j - it.n_sink + it.w0 : j; }
+__device__ __forceinline__ int tile_of(const TcWindowItem& it, int j) {
+    j += it.j0;
+    return j >= it.n_sink ? j - it.n_sink + it.w0 : j;
+}
 
 constexpr int kMaxCachedItems = 32;  // work items of a CTA kept in shared memory (later rounds are derived on the fly)
 
@@ -228,7 +261,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     // (round r left to right when even, right to left when odd), which keeps the summed causal work
     // per CTA within about one K/V step of the mean.  Tree: equal items, same dealing.
     const int n_items = kTree ? p.batch * p.num_kv_heads * p.units_per_kvh
-                              : p.n_qblocks * p.batch * p.num_kv_heads * p.units_per_kvh;
+                              : p.n_qblocks * p.batch * p.num_kv_heads * p.units_per_kvh * (kWindow ? p.n_chunks : 1);
     const int n_rounds = (n_items + (int)gridDim.x - 1) / (int)gridDim.x;
     auto derive_item = [&](int r) {
         Item it;
@@ -254,6 +287,10 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             it.q0 = 0;
             it.rows_here = kT;
         } else {
+            if constexpr (kWindow) {
+                it.chunk = pp % p.n_chunks;
+                pp /= p.n_chunks;
+            }
             // pp = qblock_rank * batch + b: the heaviest query blocks of every sequence come first
             it.b = pp % p.batch;
             pp /= p.batch;
@@ -263,13 +300,13 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             const int k_end = min(p.seq_kv, p.start_pos + it.q0 + it.rows_here);  // exclusive: last visible key + 1
             it.n_steps = (k_end + kT - 1) / kT;
             if constexpr (kWindow) {
-                const int first_pos = p.start_pos + it.q0;
-                it.lo = window_span(first_pos, p.window, p.sinks).lo;
-                const int tiles = it.n_steps;
-                it.w0 = min(it.lo / kT, tiles);
-                it.n_sink = min((min(p.sinks, it.lo) + kT - 1) / kT, it.w0);
-                it.n_steps = max(it.n_sink + tiles - it.w0, 1);  // (a block that sees nothing still runs one, masked, step)
-                if (it.n_sink + tiles - it.w0 < 1) it.w0 = 0;
+                const WindowSteps w = window_steps(p, it.q0);
+                it.lo = w.lo;
+                it.w0 = w.w0;
+                it.n_sink = w.n_sink;
+                it.j0 = chunk_begin(w.n, p.n_chunks, it.chunk);
+                it.n_steps = chunk_begin(w.n, p.n_chunks, it.chunk + 1) - it.j0;
+                it.valid = it.valid && it.n_steps > 0;
             }
             it.n_prefix = it.n_steps;
             it.cache_len = p.seq_kv;  // paged K/V: pages past the live length are not looked up
@@ -595,7 +632,8 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             __syncwarp();
             tmem_ld_16x256b_x8(e.o_frag + h * 64, rr);
             tmem_wait_ld();
-            if (!kTree && p.out_fp16) {
+            const bool partial = kWindow && p.n_chunks > 1;
+            if (!kTree && p.out_fp16 && !partial) {
                 // a thread holds pairs of columns; a 4 x 4 exchange inside the quad turns four pairs of
                 // one 8-column group into one 16-byte piece per lane: the quad then writes 64
                 // contiguous bytes of a row per store instruction
@@ -615,7 +653,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     }
                 }
             } else {
-                float* outp = kTree ? p.tree_out : static_cast<float*>(p.out);
+                float* outp = kTree ? p.tree_out : partial ? p.part_o : static_cast<float*>(p.out);
 #pragma unroll
                 for (int r = 0; r < 2; r++)
                     if (e.store[r]) {
@@ -909,6 +947,14 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     } else {
                         e.store[q] = row_of[q] < it.rows_here;
                         e.base[q] = (((size_t)it.b * p.seq_q + it.q0 + row_of[q]) * p.num_heads + it.head0 + t) * hd;
+                        if constexpr (kWindow) {
+                            if (p.n_chunks > 1) {  // the chunk's partial as it stands
+                                e.inv[q] = kQ8 ? p.v_max[it.kvh] : 1.f;
+                                const size_t at = (((size_t)it.b * p.seq_q + it.q0 + row_of[q]) * p.num_heads + it.head0 + t) * p.n_chunks + it.chunk;
+                                e.base[q] = at * hd;
+                                if (tq == 0 && e.store[q]) p.part_ml[at] = make_float2(m_used_t[t][q], l);
+                            }
+                        }
                     }
                 }
                 if (kDefer) {
@@ -952,6 +998,88 @@ static int launch_tc(granite_cuda_compute* c, TcKernel kern, const char* name, i
     return GRANITE_CUDA_SUCCESS;
 }
 
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the chunks of a row, in chunk order; one warp per (row, head).
+constexpr int kMaxChunks = 32;  // one per lane
+__global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constant__ TcParams p, int hd) {
+    const int lane = threadIdx.x & 31;
+    const size_t idx = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);  // (sequence, row, head)
+    const size_t total = (size_t)p.batch * p.seq_q * p.num_heads;
+    if (idx >= total) return;
+    const int row = (int)(idx / p.num_heads % p.seq_q);
+    const int n = window_steps(p, row / kT * kT).n;
+    const bool has = lane < p.n_chunks && chunk_begin(n, p.n_chunks, lane + 1) > chunk_begin(n, p.n_chunks, lane);  // (an empty chunk wrote nothing)
+    const float2 ml = has ? p.part_ml[idx * p.n_chunks + lane] : make_float2(-INFINITY, 0.f);
+    float M = ml.x;
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, sh));
+    const float w = has ? fast_exp2(ml.x - M) : 0.f;
+    float L = w * ml.y;
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) L += __shfl_xor_sync(0xffffffffu, L, sh);
+    const float inv = L > 0.f ? 1.f / L : 0.f;  // a row that sees nothing is zero
+    const bool col = lane * 4 < hd;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < p.n_chunks; c++) {
+        const float wc = __shfl_sync(0xffffffffu, w, c);
+        if (!__shfl_sync(0xffffffffu, (int)has, c) || !col) continue;
+        const float4 o = *reinterpret_cast<const float4*>(p.part_o + (idx * p.n_chunks + c) * hd + lane * 4);
+        acc.x = fmaf(wc, o.x, acc.x);
+        acc.y = fmaf(wc, o.y, acc.y);
+        acc.z = fmaf(wc, o.z, acc.z);
+        acc.w = fmaf(wc, o.w, acc.w);
+    }
+    if (!col) return;
+    acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (p.out_fp16)
+        *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + idx * hd + lane * 4) = make_uint2(pack_half2(acc.x, acc.y), pack_half2(acc.z, acc.w));
+    else
+        *reinterpret_cast<float4*>(static_cast<float*>(p.out) + idx * hd + lane * 4) = acc;
+}
+
+// How many chunks an item's tiles are cut into.  The estimate is the longest queue of any SM - items come in rounds of one per
+// SM, a chunk costs its steps and about one and a half more to start and drain - plus the merge's launch and traffic, at
+// 1.35 us a step.  An fp32 output additionally wants no more than 22 tiles in one accumulator (see the top of the file).
+// Returns the bytes of partials; fills n_chunks.
+static size_t plan_chunks(granite_cuda_compute* c, TcParams& p, int hd) {
+    const long long items = (long long)p.n_qblocks * p.batch * p.num_kv_heads * p.units_per_kvh;
+    int longest = 1;
+    for (int b = 0; b < p.n_qblocks; b += 1 + p.n_qblocks / 64) longest = std::max(longest, window_steps(p, b * kT).n);
+    longest = std::max(longest, window_steps(p, (p.n_qblocks - 1) * kT).n);
+    const double rows = (double)p.batch * p.seq_q * p.num_heads;
+    double best = 0;
+    p.n_chunks = 1;
+    static const int choices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, kMaxChunks};
+    bool chosen = false;
+    for (int n : choices) {
+        if (n > longest || items * n >= (1ll << 31)) break;
+        const int steps = (longest + n - 1) / n;
+        if (!p.out_fp16 && steps > 22 && n < kMaxChunks && n < longest) continue;
+        const double rounds = (double)((items * n + c->sm_count - 1) / c->sm_count);
+        const double us = rounds * (steps + 1.5) * 1.35 + (n > 1 ? 3.0 + rows * n * hd * 8 / 5e6 : 0.0);
+        if (!chosen || us < best) {
+            best = us;
+            p.n_chunks = n;
+            chosen = true;
+        }
+    }
+    if (p.n_chunks == 1) return 0;
+    return (size_t)rows * p.n_chunks * (hd * 4 + sizeof(float2)) + 256;
+}
+static void place_partials(TcParams& p, uint8_t* at, int hd) {
+    if (p.n_chunks == 1) return;
+    const size_t n = (size_t)p.batch * p.seq_q * p.num_heads * p.n_chunks;
+    p.part_o = reinterpret_cast<float*>(at);
+    p.part_ml = reinterpret_cast<float2*>(at + n * hd * 4);
+}
+static int launch_merge(granite_cuda_compute* c, const TcParams& p, int hd) {
+    if (p.n_chunks <= 1) return GRANITE_CUDA_SUCCESS;
+    const size_t warps = (size_t)p.batch * p.seq_q * p.num_heads;
+    LaunchScope t(c, "prefill_merge");
+    prefill_merge_kernel<<<(unsigned)((warps + 7) / 8), 256, 0, c->stream>>>(p, hd);
+    GB_CUDA_TRY(cudaGetLastError());
+    return GRANITE_CUDA_SUCCESS;
+}
+
 static void set_window(TcParams& p, const CacheView& view) {
     p.window = (int)std::min(view.window, 0x7fffffffu);
     p.sinks = (int)std::min(view.sinks, 0x7fffffffu);
@@ -990,12 +1118,6 @@ int launch_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, c
     if ((uint64_t)batch * a.seq_q >= (1ull << 31) || (uint64_t)batch * a.num_kv_heads * max_seq >= (1ull << 31))
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, "prefill: batch * rows exceeds the tensor-map coordinate range");
 
-    const bool split_q = a.q_dtype == 0;
-    const void *q16 = a.q, *q16_lo = a.q;
-    if (split_q) {
-        int rc = split_queries(c, a.q, (size_t)batch * a.seq_q * a.num_heads * D, &q16, &q16_lo);
-        if (rc) return rc;
-    }
     TcParams p{};
     p.d_chunks = (int)D / 64;
     p.batch = (int)batch;
@@ -1014,6 +1136,21 @@ int launch_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, c
     p.n_qblocks = (p.seq_q + kT - 1) / kT;
     p.start_pos = (int)a.start_pos;
 
+    p.n_chunks = 1;
+    size_t partials = 0;
+    if (view.window > 0) {
+        set_window(p, view);
+        partials = plan_chunks(c, p, (int)D);
+    }
+    const bool split_q = a.q_dtype == 0;
+    const void *q16 = a.q, *q16_lo = a.q;
+    const size_t n_q = (size_t)batch * a.seq_q * a.num_heads * D;
+    if (split_q || partials) {
+        int rc = split_q ? split_queries(c, a.q, n_q, &q16, &q16_lo, partials) : c->ensure_scratch(partials);
+        if (rc) return rc;
+        place_partials(p, static_cast<uint8_t*>(c->scratch) + (split_q ? split_bytes(n_q) : 0), (int)D);
+    }
+
     const uint64_t q_rows = (uint64_t)batch * a.seq_q;
     const CUtensorMap* qmap = c->tensor_map_2d(q16, (uint64_t)a.num_heads * D, q_rows, (uint64_t)a.num_heads * D * 2, 64, kT, 128);
     const CUtensorMap* qlomap = c->tensor_map_2d(q16_lo, (uint64_t)a.num_heads * D, q_rows, (uint64_t)a.num_heads * D * 2, 64, kT, 128);
@@ -1023,12 +1160,10 @@ int launch_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, c
     if (!qmap || !qlomap || !kmap || !vmap) return GRANITE_CUDA_EXECUTION_FAILED;
 
     TcKernel kern = split_q ? fa_tc_kernel<false, false, true, 1> : fa_tc_kernel<false, false, false, 1>;
-    if (view.window > 0) {
-        set_window(p, view);
-        kern = split_q ? fa_tc_kernel<false, false, true, 1, true> : fa_tc_kernel<false, false, false, 1, true>;
-    }
-    const int n_items = p.n_qblocks * p.batch * p.num_kv_heads * p.units_per_kvh;
-    return launch_tc(c, kern, view.window > 0 ? "prefill_window_fa" : "prefill_causal_fa", n_items, split_q ? 2 : tiles, qmap, qlomap, kmap, vmap, kmap, vmap, p);
+    if (view.window > 0) kern = split_q ? fa_tc_kernel<false, false, true, 1, true> : fa_tc_kernel<false, false, false, 1, true>;
+    const int n_items = p.n_qblocks * p.batch * p.num_kv_heads * p.units_per_kvh * p.n_chunks;
+    int rc = launch_tc(c, kern, view.window > 0 ? "prefill_window_fa" : "prefill_causal_fa", n_items, split_q ? 2 : tiles, qmap, qlomap, kmap, vmap, kmap, vmap, p);
+    return rc ? rc : launch_merge(c, p, (int)D);
 }
 
 // Causal attention of a chunk of new tokens against the sequence's paged cache: the prefill
@@ -1049,12 +1184,6 @@ int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillA
     if (seq_kv > (uint64_t)a.max_blocks_per_seq * kPageRows)
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, "paged_prefill_attention: the chunk ends beyond the block table");
 
-    const bool split_q = a.q_dtype == 0;
-    const void *q16 = a.q, *q16_lo = a.q;
-    if (split_q) {
-        int rc = split_queries(c, a.q, (size_t)a.seq_q * a.num_heads * D, &q16, &q16_lo);
-        if (rc) return rc;
-    }
     TcParams p{};
     p.d_chunks = (int)D / 64;
     p.num_heads = (int)a.num_heads;
@@ -1075,6 +1204,21 @@ int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillA
     p.max_blocks = (int)a.max_blocks_per_seq;
     p.num_blocks = (int)a.num_blocks;
 
+    p.n_chunks = 1;
+    size_t partials = 0;
+    if (view.window > 0) {
+        set_window(p, view);
+        partials = plan_chunks(c, p, (int)D);
+    }
+    const bool split_q = a.q_dtype == 0;
+    const void *q16 = a.q, *q16_lo = a.q;
+    const size_t n_q = (size_t)a.seq_q * a.num_heads * D;
+    if (split_q || partials) {
+        int rc = split_q ? split_queries(c, a.q, n_q, &q16, &q16_lo, partials) : c->ensure_scratch(partials);
+        if (rc) return rc;
+        place_partials(p, static_cast<uint8_t*>(c->scratch) + (split_q ? split_bytes(n_q) : 0), (int)D);
+    }
+
     const CUtensorMap* qmap = c->tensor_map_2d(q16, (uint64_t)a.num_heads * D, a.seq_q, (uint64_t)a.num_heads * D * 2, 64, kT, 128);
     const CUtensorMap* qlomap = c->tensor_map_2d(q16_lo, (uint64_t)a.num_heads * D, a.seq_q, (uint64_t)a.num_heads * D * 2, 64, kT, 128);
     const uint64_t rows = (uint64_t)a.num_blocks * kPageRows, width = (uint64_t)a.num_kv_heads * D;
@@ -1083,12 +1227,10 @@ int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillA
     if (!qmap || !qlomap || !kmap || !vmap) return GRANITE_CUDA_EXECUTION_FAILED;
 
     TcKernel kern = split_q ? fa_tc_kernel<false, true, true, 1> : fa_tc_kernel<false, true, false, 1>;
-    if (view.window > 0) {
-        set_window(p, view);
-        kern = split_q ? fa_tc_kernel<false, true, true, 1, true> : fa_tc_kernel<false, true, false, 1, true>;
-    }
-    const int n_items = p.n_qblocks * p.num_kv_heads * p.units_per_kvh;
-    return launch_tc(c, kern, view.window > 0 ? "paged_prefill_window_fa" : "paged_prefill_fa", n_items, split_q ? 2 : 1, qmap, qlomap, kmap, vmap, kmap, vmap, p);
+    if (view.window > 0) kern = split_q ? fa_tc_kernel<false, true, true, 1, true> : fa_tc_kernel<false, true, false, 1, true>;
+    const int n_items = p.n_qblocks * p.num_kv_heads * p.units_per_kvh * p.n_chunks;
+    int rc = launch_tc(c, kern, view.window > 0 ? "paged_prefill_window_fa" : "paged_prefill_fa", n_items, split_q ? 2 : 1, qmap, qlomap, kmap, vmap, kmap, vmap, p);
+    return rc ? rc : launch_merge(c, p, (int)D);
 }
 
 // ------------------------------------------------------------------------------------ 8-bit cache
@@ -1243,11 +1385,14 @@ int launch_paged_prefill_q8(granite_cuda_compute* c, const GraniteCudaPagedPrefi
     const size_t q_bytes = split_q ? split_bytes(n_q) : 0;
     const size_t kv_bytes = (size_t)g.hkv * g.rows * D * 2;                                           // a multiple of 128 rows * 128 bytes
     const size_t page_bytes = ((size_t)g.hkv * g.page_stride * 4 + 255) / 256 * 256;
-    const size_t behind = 2 * kv_bytes + 3 * page_bytes + ((size_t)g.hkv * 4 + 255) / 256 * 256;
+    const size_t partials = plan_chunks(c, p, (int)D);
+    const size_t fixed = 2 * kv_bytes + 3 * page_bytes + ((size_t)g.hkv * 4 + 255) / 256 * 256;
+    const size_t behind = fixed + partials;
     const void *q16 = a.q, *q16_lo = a.q;
     int rc = split_q ? split_queries(c, a.q, n_q, &q16, &q16_lo, behind) : c->ensure_scratch(behind);
     if (rc) return rc;
     uint8_t* ws = static_cast<uint8_t*>(c->scratch) + q_bytes;
+    place_partials(p, ws + fixed, (int)D);
     g.k16 = reinterpret_cast<__half*>(ws);
     g.v16 = reinterpret_cast<__half*>(ws + kv_bytes);
     g.page_k = reinterpret_cast<float*>(ws + 2 * kv_bytes);
@@ -1278,8 +1423,9 @@ int launch_paged_prefill_q8(granite_cuda_compute* c, const GraniteCudaPagedPrefi
     const CUtensorMap* vmap = c->tensor_map_2d(g.v16, D, (uint64_t)g.hkv * g.rows, D * 2, 64, kT, 128);
     if (!qmap || !qlomap || !kmap || !vmap) return GRANITE_CUDA_EXECUTION_FAILED;
     TcKernel kern = split_q ? fa_tc_kernel<false, false, true, 1, true, true> : fa_tc_kernel<false, false, false, 1, true, true>;
-    const int n_items = p.n_qblocks * p.num_kv_heads * p.units_per_kvh;
-    return launch_tc(c, kern, "paged_prefill_q8_fa", n_items, split_q ? 2 : 1, qmap, qlomap, kmap, vmap, kmap, vmap, p);
+    const int n_items = p.n_qblocks * p.num_kv_heads * p.units_per_kvh * p.n_chunks;
+    rc = launch_tc(c, kern, "paged_prefill_q8_fa", n_items, split_q ? 2 : 1, qmap, qlomap, kmap, vmap, kmap, vmap, p);
+    return rc ? rc : launch_merge(c, p, (int)D);
 }
 
 int launch_tree_mask(granite_cuda_compute* c, const int32_t* parents, uint64_t* masks, uint32_t batch, uint32_t n) {
