@@ -155,6 +155,34 @@ Result<void> CudaCompute::paged_prefill_attention(const GraniteCudaPagedPrefillA
     return cuda_result(granite_cuda_paged_prefill_attention(h_, &args));
 }
 
+Result<void> CudaCompute::rope_paged_kv_cache_append_q8(const GraniteCudaRopeAppendArgs& args, const GraniteCudaQ8Cache& cache) {
+    return cuda_result(granite_cuda_rope_paged_kv_cache_append_q8(h_, &args, &cache));
+}
+
+Result<void> CudaCompute::batched_paged_attention_decode_q8(const GraniteCudaPagedDecodeArgs& args, const GraniteCudaQ8Cache& cache,
+                                                            const GraniteCudaAttentionWindow* window) {
+    return cuda_result(granite_cuda_batched_paged_attention_decode_q8(h_, &args, &cache, window));
+}
+
+Result<void> CudaCompute::paged_prefill_attention_q8(const GraniteCudaPagedPrefillArgs& args, const GraniteCudaQ8Cache& cache,
+                                                     const GraniteCudaAttentionWindow* window) {
+    return cuda_result(granite_cuda_paged_prefill_attention_q8(h_, &args, &cache, window));
+}
+
+Result<void> CudaCompute::batched_paged_attention_decode_window(const GraniteCudaPagedDecodeArgs& args,
+                                                                const GraniteCudaAttentionWindow& window) {
+    return cuda_result(granite_cuda_batched_paged_attention_decode_window(h_, &args, &window));
+}
+
+Result<void> CudaCompute::multihead_attention_window(const GraniteCudaAttentionArgs& args, const GraniteCudaAttentionWindow& window) {
+    return cuda_result(granite_cuda_multihead_attention_window(h_, &args, &window));
+}
+
+Result<void> CudaCompute::paged_prefill_attention_window(const GraniteCudaPagedPrefillArgs& args,
+                                                         const GraniteCudaAttentionWindow& window) {
+    return cuda_result(granite_cuda_paged_prefill_attention_window(h_, &args, &window));
+}
+
 // =================================================================== RoPECache (src/llm/rope.cpp)
 void RoPECache::initialize(int max_seq_len, int head_dim, float theta) {
     max_seq_len_ = max_seq_len;

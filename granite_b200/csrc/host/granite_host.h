@@ -312,6 +312,16 @@ public:
     Result<void> rope_paged_kv_cache_append(const GraniteCudaRopeAppendArgs& args);
     Result<void> tree_commit(const GraniteCudaTreeCommitArgs& args);
     Result<void> paged_prefill_attention(const GraniteCudaPagedPrefillArgs& args);
+    // The 8-bit paged cache (int8 or fp8 e4m3 codes, a scale per page and KV head) and sliding windows with sinks.
+    // No counterpart upstream; argument meaning as in granite_cuda.h (window nullptr on the q8 calls: none).
+    Result<void> rope_paged_kv_cache_append_q8(const GraniteCudaRopeAppendArgs& args, const GraniteCudaQ8Cache& cache);
+    Result<void> batched_paged_attention_decode_q8(const GraniteCudaPagedDecodeArgs& args, const GraniteCudaQ8Cache& cache,
+                                                   const GraniteCudaAttentionWindow* window = nullptr);
+    Result<void> paged_prefill_attention_q8(const GraniteCudaPagedPrefillArgs& args, const GraniteCudaQ8Cache& cache,
+                                            const GraniteCudaAttentionWindow* window = nullptr);
+    Result<void> batched_paged_attention_decode_window(const GraniteCudaPagedDecodeArgs& args, const GraniteCudaAttentionWindow& window);
+    Result<void> multihead_attention_window(const GraniteCudaAttentionArgs& args, const GraniteCudaAttentionWindow& window);
+    Result<void> paged_prefill_attention_window(const GraniteCudaPagedPrefillArgs& args, const GraniteCudaAttentionWindow& window);
 private:
     granite_cuda_compute_t* h_ = nullptr;
 };

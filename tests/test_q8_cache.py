@@ -547,6 +547,31 @@ def test_prefill_q8_refusals(kw, code, word):
     assert got.name == code and word in text
 
 
+def test_structures_match_the_header(tmp_path):
+    """GraniteCudaQ8Cache and GraniteCudaAttentionWindow as a C compiler lays them out, against the binding's."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    from granite_b200 import capi
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "granite_cuda.h"', "int main(void) {"]
+    pairs = {"GraniteCudaQ8Cache": capi.Q8Cache, "GraniteCudaAttentionWindow": capi.AttentionWindow}
+    for name, cls in pairs.items():
+        lines.append(f'  printf("{name} %zu\\n", sizeof({name}));')
+        lines += [f'  printf("{name}.{f} %zu\\n", offsetof({name}, {f}));' for f, _ in cls._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]))
+    include = Path(__file__).resolve().parent.parent / "include"
+    subprocess.run([cc, "-std=c11", f"-I{include}", str(src), "-o", str(exe)], check=True)
+    out = dict(x.split() for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines())
+    for name, cls in pairs.items():
+        assert int(out[name]) == C.sizeof(cls)
+        for f, _ in cls._fields_:
+            assert int(out[f"{name}.{f}"]) == getattr(cls, f).offset
+
+
 def test_reference_encoding_is_the_format():
     """The checker's own e4m3 rounding, on every value, every midpoint and beyond the range; torch's cast as a second opinion."""
     import torch
