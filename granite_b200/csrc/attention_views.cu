@@ -1,5 +1,7 @@
 // Attention calls that see the cache through a view - 8-bit codes with page scales, a sliding window, or both: their
 // argument checks (none of which needs a device) and the choice between the tuned and the plain kernel.
+#include <cmath>
+
 #include "compute_internal.h"
 #include "q8.cuh"
 
@@ -19,6 +21,12 @@ int check_heads(uint32_t num_heads, uint32_t num_kv_heads, uint32_t head_dim, co
     return GRANITE_CUDA_SUCCESS;
 }
 
+// (a masked score is -infinity and has to stay that when it is scaled)
+int check_scale(float scale, const std::string& what) {
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": scale must be positive and finite");
+    return GRANITE_CUDA_SUCCESS;
+}
+
 int check_pool(uint32_t block_size, uint32_t num_blocks, uint32_t max_blocks, const std::string& what) {
     if (block_size == 0 || num_blocks == 0 || max_blocks == 0) return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": empty pool or table");
     if ((uint64_t)block_size * max_blocks >= kIntLimit || (uint64_t)block_size * num_blocks >= kIntLimit)
@@ -34,6 +42,7 @@ int check_decode_view(const GraniteCudaPagedDecodeArgs& a, bool contiguous, uint
         return fail(GRANITE_CUDA_NULL_POINTER, what + ": null buffer");
     if (a.batch_size == 0) return GRANITE_CUDA_SUCCESS;
     if (int rc = check_heads(a.num_heads, a.num_kv_heads, a.head_dim, what)) return rc;
+    if (int rc = check_scale(a.scale, what)) return rc;
     if (a.batch_size > 65535) return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": at most 65535 sequences per call");
     if (unaligned16(a.q, a.output) || unaligned16(a.k_cache, a.v_cache))
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": Q, the caches and the output must be 16-byte aligned");
@@ -48,6 +57,7 @@ int check_prefill_view(const GraniteCudaAttentionArgs& a) {
     const std::string what = "prefill window";
     if (!a.q || !a.k || !a.v || !a.output) return fail(GRANITE_CUDA_NULL_POINTER, what + ": null buffer");
     if (int rc = check_heads(a.num_heads, a.num_kv_heads, a.head_dim, what)) return rc;
+    if (int rc = check_scale(a.scale, what)) return rc;
     if (a.q_dtype > 1 || a.out_dtype > 1) return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": dtype must be 0 (fp32) or 1 (fp16)");
     if (unaligned16(a.q, a.output) || unaligned16(a.k, a.v))
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": Q, K, V and the output must be 16-byte aligned");
@@ -63,6 +73,7 @@ int check_paged_prefill_view(const GraniteCudaPagedPrefillArgs& a) {
     const std::string what = "paged prefill";
     if (!a.q || !a.k_cache || !a.v_cache || !a.block_table || !a.output) return fail(GRANITE_CUDA_NULL_POINTER, what + ": null buffer");
     if (int rc = check_heads(a.num_heads, a.num_kv_heads, a.head_dim, what)) return rc;
+    if (int rc = check_scale(a.scale, what)) return rc;
     if (a.q_dtype > 1 || a.out_dtype > 1) return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": dtype must be 0 (fp32) or 1 (fp16)");
     if (unaligned16(a.q, a.output) || unaligned16(a.k_cache, a.v_cache))
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, what + ": Q, the pools and the output must be 16-byte aligned");

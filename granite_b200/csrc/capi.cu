@@ -44,28 +44,34 @@ using namespace gb200;
 
 int granite_cuda_compute::ensure_scratch(size_t bytes) {
     if (bytes <= scratch_bytes) return GRANITE_CUDA_SUCCESS;
-    // growing: make sure nothing in flight still uses the old arena
-    GB_CUDA_TRY(cudaStreamSynchronize(stream));
-    if (scratch) cudaFree(scratch);
-    scratch = nullptr;
-    scratch_bytes = 0;
+    // growing: calls in flight and captured graphs may still use the old arena, so it is kept until the object goes
     size_t want = bytes + bytes / 4;
-    cudaError_t e = cudaMalloc(&scratch, want);
-    if (e != cudaSuccess) return fail(GRANITE_CUDA_OUT_OF_MEMORY, "scratch arena: cudaMalloc failed");
+    void* grown = nullptr;
+    if (cudaMalloc(&grown, want) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(GRANITE_CUDA_OUT_OF_MEMORY, "scratch arena: cudaMalloc failed");
+    }
+    if (scratch) retired.push_back(scratch);
+    scratch = grown;
     scratch_bytes = want;
     return GRANITE_CUDA_SUCCESS;
 }
 
 int granite_cuda_compute::ensure_page_counters(size_t count) {
     if (count <= pages_done_count) return GRANITE_CUDA_SUCCESS;
-    GB_CUDA_TRY(cudaStreamSynchronize(stream));  // growing: nothing in flight may still count in the old array
-    if (d_pages_done) cudaFree(d_pages_done);
-    d_pages_done = nullptr;
-    pages_done_count = 0;
     const size_t want = count + count / 4 + 1024;
-    if (cudaMalloc(&d_pages_done, want * sizeof(int)) != cudaSuccess)
+    int* grown = nullptr;
+    if (cudaMalloc(&grown, want * sizeof(int)) != cudaSuccess) {
+        cudaGetLastError();
         return fail(GRANITE_CUDA_OUT_OF_MEMORY, "decode page counters: cudaMalloc failed");
-    GB_CUDA_TRY(cudaMemsetAsync(d_pages_done, 0, want * sizeof(int), stream));
+    }
+    if (cudaMemsetAsync(grown, 0, want * sizeof(int), stream) != cudaSuccess) {
+        cudaGetLastError();
+        cudaFree(grown);
+        return fail(GRANITE_CUDA_EXECUTION_FAILED, "decode page counters: clearing failed");
+    }
+    if (d_pages_done) retired.push_back(d_pages_done);  // (as the scratch arena)
+    d_pages_done = grown;
     pages_done_count = want;
     return GRANITE_CUDA_SUCCESS;
 }
@@ -245,6 +251,7 @@ void granite_cuda_compute_destroy(granite_cuda_compute_t* c) {
     if (c->scratch) cudaFree(c->scratch);
     if (c->d_status) cudaFree(c->d_status);
     if (c->d_pages_done) cudaFree(c->d_pages_done);
+    for (void* old : c->retired) cudaFree(old);
     if (c->h_status) cudaFreeHost(c->h_status);
     if (c->owns_stream && c->stream) cudaStreamDestroy(c->stream);
     delete c;

@@ -74,9 +74,11 @@ struct granite_cuda_compute {
     int* h_status = nullptr;  // pinned mirror
     uint64_t dispatches = 0;
     uint64_t syncs = 0;
-    // scratch arena (grown on demand, never shrunk)
+    // scratch arena (grown on demand, never shrunk; a graph captured before it grew goes on using the smaller one, which
+    // therefore lives as long as the object)
     void* scratch = nullptr;
     size_t scratch_bytes = 0;
+    std::vector<void*> retired;
     // Cached TMA descriptors, keyed by (buffer, shape).  Bounded: once kMaxTensorMaps entries exist,
     // everything but the kKeepRecent most recently used ones is dropped (encode_map), so a pointer
     // returned by encode_map stays valid for at least the next kKeepRecent - 1 calls to it.

@@ -473,6 +473,9 @@ typedef struct {
     uint32_t sinks;
 } GraniteCudaAttentionWindow;
 
+/* All calls below: Q, K, V, caches and outputs 16-byte aligned, scale positive and finite, at most 65535 heads and
+ * (decode) 65535 sequences, positions below 2^31 - 65536; anything else is refused before a device is touched. */
+
 /* granite_cuda_rope_paged_kv_cache_append into the 8-bit cache (args->k_cache / v_cache are its pools).  For every
  * (sequence, page the call touches, KV head), for K after the rotation and for V:
  *     need  = max |x| over the call's rows in the page / (127 or 448)
@@ -493,7 +496,8 @@ int granite_cuda_rope_paged_kv_cache_append_q8(granite_cuda_compute_t* c, const 
 int granite_cuda_batched_paged_attention_decode_q8(granite_cuda_compute_t* c, const GraniteCudaPagedDecodeArgs* args,
                                                    const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window);
 
-/* granite_cuda_paged_prefill_attention over the 8-bit cache; window may be NULL.  Same shapes as the fp16 call. */
+/* granite_cuda_paged_prefill_attention over the 8-bit cache; window may be NULL.  Same shapes as the fp16 call.  The visible
+ * codes are laid out as fp16 in the object's scratch first (4 bytes per key, KV head and dim). */
 int granite_cuda_paged_prefill_attention_q8(granite_cuda_compute_t* c, const GraniteCudaPagedPrefillArgs* args,
                                             const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window);
 

@@ -480,6 +480,102 @@ def test_q8_calls_replay_from_a_graph_on_another_stream():
         o.shutdown()
 
 
+@pytest.mark.gpu
+def test_a_captured_graph_outlives_the_growth_of_the_workspace():
+    """A graph holds the workspace that it was captured with; a later, larger call must not take it away."""
+    import torch
+    import granite_b200 as g
+    side = torch.cuda.Stream(device=DEV)
+    o = g.CudaCompute(0, side.cuda_stream)
+    hq, hkv, d = 32, 8, 128
+    c = _decode_case(30, [900, 1200, 40] * 20, hq, hkv, d, 0)
+    held = [_dev(c[n]) for n in ("q", "kc", "vc", "ks", "vs", "tables", "lens")]
+    out = torch.zeros(c["q"].shape, device=DEV)
+
+    def step():
+        o.batched_paged_attention_decode_q8(*held, out, len(c["lens"]), hq, hkv, d, 16, c["tables"].shape[1], c["scale"], num_blocks=c["blocks"], cache_dtype=0)
+
+    torch.cuda.synchronize()
+    step()
+    o.sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    p = _prefill_case(31, 300, 2000, 8, 2, d, 1, False)  # more workspace than the step's
+    big = _decode_case(32, [20] * 400, hq, hkv, d, 0)     # more sequences: larger counters and tables
+    p_out, b_out = torch.zeros(p["q"].shape, device=DEV), torch.zeros(big["q"].shape, device=DEV)
+    p_held = [_dev(p["q"])] + [_dev(p[n]) for n in ("kc", "vc", "ks", "vs", "tables")]
+    b_held = [_dev(big[n]) for n in ("q", "kc", "vc", "ks", "vs", "tables", "lens")]
+    torch.cuda.synchronize()
+    o.paged_prefill_attention_q8(*p_held, p_out, 8, 2, 300, 2000, d, 16, p["tables"].shape[1], p["blocks"], p["scale"], 1)
+    o.batched_paged_attention_decode_q8(*b_held, b_out, 400, hq, hkv, d, 16, big["tables"].shape[1], big["scale"], num_blocks=big["blocks"], cache_dtype=0)
+    o.sync()
+    junk = [torch.full((1 << 22,), float("nan"), device=DEV) for _ in range(8)]  # whatever memory was given back is written over
+    out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    o.sync()
+    R.assert_close(out.cpu().numpy(), c["want"], c["bound"], what="replay after growth")
+    R.assert_close(p_out.cpu().numpy(), p["want"], p["bound"], what="prefill")
+    R.assert_close(b_out.cpu().numpy(), big["want"], big["bound"], what="large batch")
+    del graph, junk
+    o.shutdown()
+
+
+@pytest.mark.gpu
+def test_two_objects_work_at_the_same_time():
+    """Two compute objects on two streams, 8-bit decode and prefill interleaved: no shared workspace, counters or status."""
+    import torch
+    import granite_b200 as g
+    streams = [torch.cuda.Stream(device=DEV) for _ in range(2)]
+    objs = [g.CudaCompute(0, s.cuda_stream) for s in streams]
+    hq, hkv, d = 16, 4, 128
+    cs = [_decode_case(40 + i, [700, 1500, 33] * 15, hq, hkv, d, i) for i in range(2)]
+    ps = [_prefill_case(50 + i, 90, 1000, hq, hkv, d, i, False) for i in range(2)]
+    held = [[_dev(c[n]) for n in ("q", "kc", "vc", "ks", "vs", "tables", "lens")] for c in cs]
+    p_held = [[_dev(p["q"])] + [_dev(p[n]) for n in ("kc", "vc", "ks", "vs", "tables")] for p in ps]
+    outs, p_outs = [torch.zeros(c["q"].shape, device=DEV) for c in cs], [torch.zeros(p["q"].shape, device=DEV) for p in ps]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i, o in enumerate(objs):
+            o.batched_paged_attention_decode_q8(*held[i], outs[i], 45, hq, hkv, d, 16, cs[i]["tables"].shape[1], cs[i]["scale"], num_blocks=cs[i]["blocks"], cache_dtype=i)
+            o.paged_prefill_attention_q8(*p_held[i], p_outs[i], hq, hkv, 90, 1000, d, 16, ps[i]["tables"].shape[1], ps[i]["blocks"], ps[i]["scale"], i)
+    for i, o in enumerate(objs):
+        o.sync()
+        R.assert_close(outs[i].cpu().numpy(), cs[i]["want"], cs[i]["bound"], what=f"decode {i}")
+        R.assert_close(p_outs[i].cpu().numpy(), ps[i]["want"], ps[i]["bound"], what=f"prefill {i}")
+        o.shutdown()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", [0, 1])
+def test_split_pages_give_the_same_bits_every_time(compute, cache_dtype):
+    """1, 2 and 4 KV heads share a head's pages among warps: many runs of the same call, long enough to wrap the ring, agree."""
+    import torch
+    for hq, hkv, d in ((16, 4, 128), (8, 2, 128), (4, 1, 128), (16, 4, 64), (4, 1, 64)):
+        c = _decode_case(60 + hkv + d, [3000, 2000, 1000, 17] * 12, hq, hkv, d, cache_dtype)
+        held = [_dev(c[n]) for n in ("q", "kc", "vc", "ks", "vs", "tables", "lens")]
+        outs = []
+        for _ in range(40):
+            out = torch.empty(c["q"].shape, device=DEV)
+            compute.batched_paged_attention_decode_q8(*held, out, len(c["lens"]), hq, hkv, d, 16, c["tables"].shape[1], c["scale"], num_blocks=c["blocks"], cache_dtype=cache_dtype)
+            outs.append(out)
+        compute.sync()
+        R.assert_close(outs[0].cpu().numpy(), c["want"], c["bound"], what=f"{hq}/{hkv}/{d}")
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype,half,seq,start,window", [(0, False, 10, 9000, 0), (1, True, 300, 5000, 0), (0, False, 140, 7000, 6000), (1, False, 1, 4097, 0)])
+def test_prefill_q8_cut_along_the_keys(compute, cache_dtype, half, seq, start, window):
+    """Few queries over many keys, and more key tiles than one accumulator takes: chunks and their merge."""
+    c = _prefill_case(seq + start, seq, start, 4, 2, 128, cache_dtype, half, window=window, sinks=3 if window else 0)
+    got = _run_prefill(compute, c, start, 2, cache_dtype, half, window=window, sinks=3 if window else 0)
+    R.assert_close(got, c["want"], c["bound"], half, f"{seq}@{start}")
+
+
 # --------------------------------------------------------------------------------------------- refusals (no device needed)
 def _refusal(fn, *args):
     from granite_b200 import capi
@@ -513,7 +609,7 @@ def test_append_q8_refusals(kw, code, word):
 def _decode_args(**kw):
     from granite_b200 import capi
     a = dict(q=256, k_cache=256, v_cache=256, block_tables=256, seq_lens=256, output=256, batch_size=1, num_heads=4, num_kv_heads=2, head_dim=128,
-             block_size=16, max_blocks_per_seq=4, num_blocks=4)
+             block_size=16, max_blocks_per_seq=4, num_blocks=4, scale=0.1)
     a.update({k: v for k, v in kw.items() if k in a})
     x = dict(k_scales=256, v_scales=256, cache_dtype=0)
     x.update({k: v for k, v in kw.items() if k in x})
@@ -526,7 +622,8 @@ VIEW_REFUSALS = [(dict(k_cache=None), "NullPointer", "null"), (dict(q=None), "Nu
                  (dict(num_heads=5), "InvalidArgument", "multiple"), (dict(num_heads=0), "InvalidArgument", "multiple"), (dict(num_kv_heads=0), "InvalidArgument", "multiple"),
                  (dict(head_dim=100), "InvalidArgument", "head_dim"), (dict(head_dim=512), "InvalidArgument", "head_dim"), (dict(k_cache=264), "InvalidArgument", "aligned"),
                  (dict(q=264), "InvalidArgument", "aligned"), (dict(num_blocks=0), "InvalidArgument", "empty"), (dict(block_size=0), "InvalidArgument", "empty"),
-                 (dict(max_blocks_per_seq=1 << 28), "InvalidArgument", "2^31"), (dict(), "NullPointer", "compute object")]
+                 (dict(max_blocks_per_seq=1 << 28), "InvalidArgument", "2^31"), (dict(scale=-0.1), "InvalidArgument", "scale"), (dict(scale=0.0), "InvalidArgument", "scale"),
+                 (dict(scale=float("nan")), "InvalidArgument", "scale"), (dict(scale=float("inf")), "InvalidArgument", "scale"), (dict(), "NullPointer", "compute object")]
 
 
 @pytest.mark.parametrize("kw,code,word", VIEW_REFUSALS)
@@ -540,7 +637,7 @@ def test_decode_q8_refusals(kw, code, word):
 def test_prefill_q8_refusals(kw, code, word):
     from granite_b200 import capi
     a = dict(q=256, k_cache=256, v_cache=256, block_table=256, output=256, num_heads=4, num_kv_heads=2, seq_q=4, start_pos=0, head_dim=128, block_size=16,
-             max_blocks_per_seq=4, num_blocks=4)
+             max_blocks_per_seq=4, num_blocks=4, scale=0.1)
     a.update({k: v for k, v in kw.items() if k in a or k == "q_dtype"})
     _, x, w = _decode_args(**kw)
     got, text = _refusal(capi.lib.granite_cuda_paged_prefill_attention_q8, C.byref(capi.PagedPrefillArgs(**a)), x, w)

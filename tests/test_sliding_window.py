@@ -218,7 +218,7 @@ def _window(kw):
 def test_decode_window_refusals(kw, code, word):
     from granite_b200 import capi
     a = dict(q=256, k_cache=256, v_cache=256, block_tables=256, seq_lens=256, output=256, batch_size=1, num_heads=4, num_kv_heads=2, head_dim=128,
-             block_size=16, max_blocks_per_seq=4, num_blocks=4)
+             block_size=16, max_blocks_per_seq=4, num_blocks=4, scale=0.1)
     a.update({k: v for k, v in kw.items() if k in a})
     got, text = _refusal(capi.lib.granite_cuda_batched_paged_attention_decode_window, C.byref(capi.PagedDecodeArgs(**a)), _window(kw))
     assert got.name == code and word in text
@@ -229,7 +229,7 @@ def test_decode_window_refusals(kw, code, word):
                                                    (dict(seq_kv=0), "InvalidArgument", "max_seq"), (dict(q_dtype=2), "InvalidArgument", "")])
 def test_multihead_window_refusals(kw, code, word, seq_q):
     from granite_b200 import capi
-    a = dict(q=256, k=256, v=256, output=256, num_heads=4, num_kv_heads=2, seq_q=seq_q, seq_kv=8, head_dim=128)
+    a = dict(q=256, k=256, v=256, output=256, num_heads=4, num_kv_heads=2, seq_q=seq_q, seq_kv=8, head_dim=128, scale=0.1)
     a.update({k: v for k, v in kw.items() if k != "window"})
     got, text = _refusal(capi.lib.granite_cuda_multihead_attention_window, C.byref(capi.AttentionArgs(**a)), _window(kw))
     assert got.name == code and word in text
@@ -237,7 +237,7 @@ def test_multihead_window_refusals(kw, code, word, seq_q):
 
 def test_prefill_window_positions_stay_in_range():
     from granite_b200 import capi
-    a = dict(q=256, k=256, v=256, output=256, num_heads=4, num_kv_heads=2, seq_q=8, seq_kv=8, head_dim=128, start_pos=0x7ffffffc)
+    a = dict(q=256, k=256, v=256, output=256, num_heads=4, num_kv_heads=2, seq_q=8, seq_kv=8, head_dim=128, start_pos=0x7ffffffc, scale=0.1)
     got, text = _refusal(capi.lib.granite_cuda_multihead_attention_window, C.byref(capi.AttentionArgs(**a)), _window({}))
     assert got.name == "InvalidArgument" and "2^31" in text
 
@@ -246,7 +246,7 @@ def test_prefill_window_positions_stay_in_range():
 def test_paged_prefill_window_refusals(kw, code, word):
     from granite_b200 import capi
     a = dict(q=256, k_cache=256, v_cache=256, block_table=256, output=256, num_heads=4, num_kv_heads=2, seq_q=4, start_pos=0, head_dim=128, block_size=16,
-             max_blocks_per_seq=4, num_blocks=4)
+             max_blocks_per_seq=4, num_blocks=4, scale=0.1)
     a.update({k: v for k, v in kw.items() if k in a})
     got, text = _refusal(capi.lib.granite_cuda_paged_prefill_attention_window, C.byref(capi.PagedPrefillArgs(**a)), _window(kw))
     assert got.name == code and word in text
