@@ -712,13 +712,13 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                 const bool need_mask = kTree ? (!tree_step && k0 + kT > it.cache_len)
                                              : ((k0 + kT - 1 > p.start_pos + it.q0) || (k0 + kT > p.seq_kv) ||
                                                 (kWindow && p.window > 0 && k0 < p.start_pos + it.q0 + kT - p.window && k0 + kT > p.sinks));
-                float page_k[kQ8 ? 8 : 1], page_lv[kQ8 ? 8 : 1];
-                const float* page_iv = nullptr;
+                float page_k[kQ8 ? 8 : 1], page_lv[kQ8 ? 8 : 1], page_iv[kQ8 ? 8 : 1];
                 if constexpr (kQ8) {
                     const size_t at = (size_t)it.kvh * p.page_stride + (size_t)(k0 / kPageRows);
-                    page_iv = p.page_iv + at;
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
+                        const float4 iv = __ldg(reinterpret_cast<const float4*>(p.page_iv + at) + c);
+                        page_iv[4 * c] = iv.x; page_iv[4 * c + 1] = iv.y; page_iv[4 * c + 2] = iv.z; page_iv[4 * c + 3] = iv.w;
                         const float4 a = __ldg(reinterpret_cast<const float4*>(p.page_k + at) + c), b = __ldg(reinterpret_cast<const float4*>(p.page_lv + at) + c);
                         page_k[4 * c] = a.x; page_k[4 * c + 1] = a.y; page_k[4 * c + 2] = a.z; page_k[4 * c + 3] = a.w;
                         page_lv[4 * c] = b.x; page_lv[4 * c + 1] = b.y; page_lv[4 * c + 2] = b.z; page_lv[4 * c + 3] = b.w;
@@ -840,7 +840,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             if constexpr (kQ8) {
 #pragma unroll
                             for (int pg = 0; pg < 4; pg++) {
-                                const float iv = __ldg(page_iv + 4 * h + pg);
+                                const float iv = page_iv[4 * h + pg];
                                 const uint64_t iv2 = f32x2(iv, iv), k2 = f32x2(page_k[4 * h + pg], page_k[4 * h + pg]);
 #pragma unroll
                                 for (int q = 0; q < 2; q++) {
@@ -1008,6 +1008,7 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constan
     const int row = (int)(idx / p.num_heads % p.seq_q);
     const int n = window_steps(p, row / kT * kT).n;
     const bool has = lane < p.n_chunks && chunk_begin(n, p.n_chunks, lane + 1) > chunk_begin(n, p.n_chunks, lane);  // (an empty chunk wrote nothing)
+    const uint32_t present = __ballot_sync(0xffffffffu, has);
     const float2 ml = has ? p.part_ml[idx * p.n_chunks + lane] : make_float2(-INFINITY, 0.f);
     float M = ml.x;
 #pragma unroll
@@ -1019,14 +1020,21 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constan
     const float inv = L > 0.f ? 1.f / L : 0.f;  // a row that sees nothing is zero
     const bool col = lane * 4 < hd;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < p.n_chunks; c++) {
-        const float wc = __shfl_sync(0xffffffffu, w, c);
-        if (!__shfl_sync(0xffffffffu, (int)has, c) || !col) continue;
-        const float4 o = *reinterpret_cast<const float4*>(p.part_o + (idx * p.n_chunks + c) * hd + lane * 4);
-        acc.x = fmaf(wc, o.x, acc.x);
-        acc.y = fmaf(wc, o.y, acc.y);
-        acc.z = fmaf(wc, o.z, acc.z);
-        acc.w = fmaf(wc, o.w, acc.w);
+    for (int c0 = 0; c0 < p.n_chunks; c0 += 4) {  // four loads in flight
+        float4 o[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            o[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (col && ((present >> (c0 + q)) & 1u)) o[q] = __ldcs(reinterpret_cast<const float4*>(p.part_o + (idx * p.n_chunks + c0 + q) * hd + lane * 4));
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const float wc = __shfl_sync(0xffffffffu, w, (c0 + q) & 31);
+            acc.x = fmaf(wc, o[q].x, acc.x);
+            acc.y = fmaf(wc, o[q].y, acc.y);
+            acc.z = fmaf(wc, o[q].z, acc.z);
+            acc.w = fmaf(wc, o[q].w, acc.w);
+        }
     }
     if (!col) return;
     acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
