@@ -31,7 +31,8 @@
 // warp does per element decides.  ldmatrix moves pairs of codes as if they were fp16 elements, which is all the two products
 // need: a product is free in how it numbers its contracted and its output dims.  For K a lane gets four consecutive dims of
 // its token per 16-dim unit, and Q is loaded in that order; for V (transposed) it gets two neighbouring dims of two tokens,
-// which are two rows of the output tile.  Code pairs become fp16 pairs in registers, exactly.  A page's K scale
+// which are two rows of the output tile.  Code pairs become fp16 pairs in registers, exactly (int8 scores need not: they
+// are integer products with the digits of Q).  A page's K scale
 // multiplies its fp32 scores; its V scale multiplies the weights, relative to a power of two that follows the largest V scale
 // seen (so weights stay bounded), and that power multiplies the accumulators at the end.  The scales of 32 pages are
 // loaded at a time, one page per lane, one batch ahead of use.
@@ -536,6 +537,9 @@ __device__ __forceinline__ void q8_pairs(uint32_t w, uint32_t& lo, uint32_t& hi)
         hi = *reinterpret_cast<const uint32_t*>(&y);
     }
 }
+// |i| < 2^22, exactly: added to the bits of 1.5 * 2^23 it is that number plus i.
+__device__ __forceinline__ float small_int_to_float(int i) { return __int_as_float(0x4B400000 + i) - 12582912.f; }
+
 // The scales of up to 32 listed pages, one per lane, and the entries of the batch after them: the chain table entry ->
 // scale is two trips to memory, so entries are fetched two batches ahead and scales one.
 struct ScaleBatch {
@@ -766,10 +770,64 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
             scales_of(e1, sb.k_next, sb.v_next);
         }
 
+        // int8: Q as three signed digits of 8 bits, q = step * (65536 d0 + 256 d1 + d2) with step = max |q| of the head / 8355584 (so
+        // that a rounding upwards still fits: the digits end at 65536 * 127 + 256 * 127 + 127 = 8355711).
+        // A digit's product with the codes is exact in 32-bit integers, on instructions that take the codes as they lie in
+        // the cache; the three sums are joined in fp32.  Columns of the n-tiles: eight heads of one digit each, or (kPair)
+        // d0 | d1 of four heads and d2 | nothing.
+        constexpr int kDigitTiles = kPair ? 2 : 3 * NT;
+        uint32_t qd[kElem == kElemInt8 ? kDigitTiles : 1][kDSteps / 2][2];
+        float q_step[NT][2];  // of the heads of the lane's score columns
+        if constexpr (kElem == kElemInt8) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const int n = kPair ? (g & 3) : nt * 8 + g;
+                const bool valid = n < n_q;
+                const float4* qp = reinterpret_cast<const float4*>(p.q + ((size_t)seg.seq * p.num_heads + hq0 + (valid ? n : 0)) * D) + t;
+                float4 qv[kDSteps];
+                float big = 0.f;
+#pragma unroll
+                for (int u = 0; u < kDSteps; u++) {  // dims 16 u + 4 t .. + 3
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (valid) v = qp[4 * u];
+                    v.x *= p.scale_log2;
+                    v.y *= p.scale_log2;
+                    v.z *= p.scale_log2;
+                    v.w *= p.scale_log2;
+                    big = fmaxf(fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                    qv[u] = v;
+                }
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                const float step = big / 8355584.f, inv = big > 0.f ? 8355584.f / big : 0.f;
+#pragma unroll
+                for (int c = 0; c < 2; c++) q_step[nt][c] = __shfl_sync(0xffffffffu, step, (kPair ? (2 * t + c) & 3 : 2 * t + c) * 4);
+#pragma unroll
+                for (int u = 0; u < kDSteps; u++) {
+                    uint32_t d[3] = {0u, 0u, 0u};
+                    const float f[4] = {qv[u].x, qv[u].y, qv[u].z, qv[u].w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int q = __float2int_rn(f[e] * inv), d2 = (int)(int8_t)q, q1 = (q - d2) >> 8, d1 = (int)(int8_t)q1, d0 = (q1 - d1) >> 8;
+                        d[0] |= (uint32_t)(d0 & 0xFF) << (8 * e);
+                        d[1] |= (uint32_t)(d1 & 0xFF) << (8 * e);
+                        d[2] |= (uint32_t)(d2 & 0xFF) << (8 * e);
+                    }
+                    if constexpr (kPair) {
+                        qd[0][u / 2][u & 1] = g < 4 ? d[0] : d[1];
+                        qd[1][u / 2][u & 1] = g < 4 ? d[2] : 0u;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 3; k++) qd[3 * nt + k][u / 2][u & 1] = d[k];
+                    }
+                }
+            }
+        }
+
         // Q^T as the B operand: lane (g,t) holds head nt*8+g, dims ks*16 + {2t,2t+1, 2t+8,2t+9}
         uint32_t qhi[NT][kDSteps][2], qlo[NT][kDSteps][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
+        for (int nt = 0; nt < (kElem == kElemInt8 ? 0 : NT); nt++) {
             const int n = kPair ? (g & 3) : nt * 8 + g;
             const bool valid = n < n_q;
             const float* qp = p.q + ((size_t)seg.seq * p.num_heads + hq0 + (valid ? n : 0)) * D;
@@ -861,14 +919,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                 }
                 const float k_scale = __shfl_sync(0xffffffffu, sb.k, j & 31), v_weight = __shfl_sync(0xffffffffu, sb.v, j & 31);
 
-                // ---- S^T = K Q^T, two 16-dim units per ldmatrix, two independent MMA chains
+                // ---- S^T = K Q^T, two 16-dim units per ldmatrix, independent MMA chains
                 float s0[NT][4] = {}, s1[NT][4] = {};
+                int sd[kElem == kElemInt8 ? kDigitTiles : 1][4] = {};
                 ok &= mbar_wait(&full[at_k], ph_k, abort_flag);
                 __syncwarp();
 #pragma unroll
                 for (int u = 0; u < kDSteps; u += 2) {
                     uint32_t w[4];  // tokens g and g + 8, units u and u + 1
                     ldmatrix_x4(w, smem_base + at_k * slot_bytes + q8_unit<D>(k_row, u + k_unit));
+                    if constexpr (kElem == kElemInt8) {
+#pragma unroll
+                        for (int k = 0; k < kDigitTiles; k++) mma_16832_s8(sd[k], w, qd[k][u / 2][0], qd[k][u / 2][1]);
+                    } else
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         uint32_t a[4];
@@ -896,8 +959,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        float v = s0[nt][i] + s1[nt][i];
+                        float v;
+                        if constexpr (kElem == kElemInt8) {
+                            // (a digit's sum is below 2^21: exact)
+                            if (kPair) v = t < 2 ? fmaf(small_int_to_float(sd[0][i]), 65536.f, small_int_to_float(sd[1][i])) : 256.f * small_int_to_float(sd[0][i]);
+                            else v = fmaf(small_int_to_float(sd[3 * nt][i]), 65536.f, fmaf(small_int_to_float(sd[3 * nt + 1][i]), 256.f, small_int_to_float(sd[3 * nt + 2][i])));
+                        } else {
+                            v = s0[nt][i] + s1[nt][i];
+                        }
                         if (kPair) v += __shfl_xor_sync(0xffffffffu, v, 2);
+                        if constexpr (kElem == kElemInt8) v *= q_step[nt][i & 1];
                         x[nt][i] = (i < 2 ? seen0 : seen1) ? v * k_scale : -INFINITY;
                         grow |= x[nt][i] > m_run[nt][i & 1] + 8.f;
                     }
