@@ -42,19 +42,36 @@ static EncodeTiledFn encode_tiled_fn() {
 
 using namespace gb200;
 
+// An allocation that is replaced by a larger one: freed once the calls in flight are done, or kept until the object goes when
+// a captured graph may hold it.
+int granite_cuda_compute::retire(void* old) {
+    if (!old) return GRANITE_CUDA_SUCCESS;
+    if (captured) {
+        retired.push_back(old);
+        return GRANITE_CUDA_SUCCESS;
+    }
+    GB_CUDA_TRY(cudaStreamSynchronize(stream));
+    GB_CUDA_TRY(cudaFree(old));
+    return GRANITE_CUDA_SUCCESS;
+}
+
 int granite_cuda_compute::ensure_scratch(size_t bytes) {
+    if (!captured) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(stream, &st) != cudaSuccess) cudaGetLastError();
+        captured = st == cudaStreamCaptureStatusActive;
+    }
     if (bytes <= scratch_bytes) return GRANITE_CUDA_SUCCESS;
-    // growing: calls in flight and captured graphs may still use the old arena, so it is kept until the object goes
     size_t want = bytes + bytes / 4;
     void* grown = nullptr;
     if (cudaMalloc(&grown, want) != cudaSuccess) {
         cudaGetLastError();
         return fail(GRANITE_CUDA_OUT_OF_MEMORY, "scratch arena: cudaMalloc failed");
     }
-    if (scratch) retired.push_back(scratch);
+    void* old = scratch;
     scratch = grown;
     scratch_bytes = want;
-    return GRANITE_CUDA_SUCCESS;
+    return retire(old);
 }
 
 int granite_cuda_compute::ensure_page_counters(size_t count) {
@@ -70,10 +87,10 @@ int granite_cuda_compute::ensure_page_counters(size_t count) {
         cudaFree(grown);
         return fail(GRANITE_CUDA_EXECUTION_FAILED, "decode page counters: clearing failed");
     }
-    if (d_pages_done) retired.push_back(d_pages_done);  // (as the scratch arena)
+    void* old = d_pages_done;
     d_pages_done = grown;
     pages_done_count = want;
-    return GRANITE_CUDA_SUCCESS;
+    return retire(old);
 }
 
 const CUtensorMap* granite_cuda_compute::encode_map(const TensorMapKey& key) {

@@ -75,10 +75,12 @@ struct granite_cuda_compute {
     uint64_t dispatches = 0;
     uint64_t syncs = 0;
     // scratch arena (grown on demand, never shrunk; a graph captured before it grew goes on using the smaller one, which
-    // therefore lives as long as the object)
+    // then lives as long as the object)
     void* scratch = nullptr;
     size_t scratch_bytes = 0;
+    bool captured = false;  // a call has been made while the stream was capturing
     std::vector<void*> retired;
+    int retire(void* old);
     // Cached TMA descriptors, keyed by (buffer, shape).  Bounded: once kMaxTensorMaps entries exist,
     // everything but the kKeepRecent most recently used ones is dropped (encode_map), so a pointer
     // returned by encode_map stays valid for at least the next kKeepRecent - 1 calls to it.

@@ -1061,6 +1061,7 @@ static size_t plan_chunks(granite_cuda_compute* c, TcParams& p, int hd) {
     bool chosen = false;
     for (int n : choices) {
         if (n > longest || items * n >= (1ll << 31)) break;
+        if (n > 1 && rows * n * (hd * 4 + 8) > 16e9) break;  // partials of more than 16 GB: the accuracy of a long run instead
         const int steps = (longest + n - 1) / n;
         if (!p.out_fp16 && steps > 22 && n < kMaxChunks && n < longest) continue;
         const double rounds = (double)((items * n + c->sm_count - 1) / c->sm_count);

@@ -785,7 +785,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                 const bool valid = n < n_q;
                 const float4* qp = reinterpret_cast<const float4*>(p.q + ((size_t)seg.seq * p.num_heads + hq0 + (valid ? n : 0)) * D) + t;
                 float4 qv[kDSteps];
-                float big = 0.f;
+                float big = 0.f, z = 0.f;  // z: NaN once a value is not finite
 #pragma unroll
                 for (int u = 0; u < kDSteps; u++) {  // dims 16 u + 4 t .. + 3
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -795,11 +795,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                     v.z *= p.scale_log2;
                     v.w *= p.scale_log2;
                     big = fmaxf(fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                    z = fmaf(v.x, 0.f, fmaf(v.y, 0.f, fmaf(v.z, 0.f, fmaf(v.w, 0.f, z))));
                     qv[u] = v;
                 }
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                const float step = big / 8355584.f, inv = big > 0.f ? 8355584.f / big : 0.f;
+                z += __shfl_xor_sync(0xffffffffu, z, 1);
+                z += __shfl_xor_sync(0xffffffffu, z, 2);
+                const float step = big / 8355584.f + z, inv = big > 0.f ? 8355584.f / big : 0.f;
 #pragma unroll
                 for (int c = 0; c < 2; c++) q_step[nt][c] = __shfl_sync(0xffffffffu, step, (kPair ? (2 * t + c) & 3 : 2 * t + c) * 4);
 #pragma unroll

@@ -318,6 +318,25 @@ def test_decode_q8_extreme_scales(compute, cache_dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("cache_dtype", [0, 1])
+def test_decode_q8_queries_out_of_the_ordinary(compute, cache_dtype):
+    """Queries of zeros and of very small and large magnitude come out right, a NaN or infinity stays in its own head."""
+    hq, hkv, d = 8, 2, 128
+    c = _decode_case(70, [100, 333], hq, hkv, d, cache_dtype)
+    q = c["q"].copy()
+    q[0, 0], q[0, 1], q[0, 2] = 0, q[0, 1] * 1e-25, q[0, 2] * 8
+    q[1, 3, 7], q[1, 5, 0] = np.nan, np.inf
+    kv, vv = R.pool_values(c["kc"], c["ks"], cache_dtype, 16), R.pool_values(c["vc"], c["vs"], cache_dtype, 16)
+    got = _run_decode(compute, dict(c, q=q), hq, hkv, d, cache_dtype)
+    assert np.isnan(got[1, 3]).all() and not np.isfinite(got[1, 5]).any()
+    for b, n in enumerate(c["lens"]):
+        fine = [h for h in range(hq) if np.isfinite(q[b, h]).all()]
+        finite = np.where(np.isfinite(q[b:b + 1]), q[b:b + 1], 0).astype(np.float64)
+        o, e = R.attend(finite, R.rows_of(kv, c["tables"][b], n, 16), R.rows_of(vv, c["tables"][b], n, 16), [n - 1], c["scale"])
+        R.assert_close(got[b][fine], o[0][fine], e[0][fine], what=f"sequence {b}")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", [0, 1])
 def test_decode_q8_reports_bad_tables_and_lengths(compute, cache_dtype):
     """Entries outside the pool and lengths outside the table are reported, not followed; the other sequences come out right."""
     from granite_b200.capi import ErrorCode, GraniteCudaError

@@ -166,6 +166,29 @@ def test_a_window_that_hides_nothing_is_the_plain_call(compute):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(16, 4, 128), (8, 2, 128), (4, 1, 128), (16, 4, 64), (8, 2, 64), (4, 1, 64), (24, 2, 64)])
+def test_split_pages_of_the_fp16_cache(compute, hq, hkv, d):
+    """The plain call and the windowed one where warps share a head's pages: ragged lengths that start segments at odd places of
+    the ring and wrap it many times; every run gives the same bits."""
+    import torch
+    lens = [3001, 17, 2000, 1, 999, 16, 48, 2500, 33] * 6
+    for window, sinks in ((0, 0), (1000, 20)):
+        q, k, v, tables, ln, blocks, want, bound = _decode_case(hkv + d, lens, hq, hkv, d, window, sinks)
+        held = [_dev(x) for x in (q, k, v, tables, ln)]
+        outs = []
+        for _ in range(25):
+            out = torch.empty(q.shape, device=DEV)
+            if window:
+                compute.batched_paged_attention_decode_window(*held, out, len(lens), hq, hkv, d, 16, tables.shape[1], d ** -0.5, window, sinks, num_blocks=blocks)
+            else:
+                compute.batched_paged_attention_decode(*held, out, len(lens), hq, hkv, d, 16, tables.shape[1], d ** -0.5, num_blocks=blocks)
+            outs.append(out)
+        compute.sync()
+        R.assert_close(outs[0].cpu().numpy(), want, bound, what=f"{hq}/{hkv}/{d} {window}")
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.gpu
 def test_window_calls_replay_from_a_graph():
     import torch
     import granite_b200 as g
