@@ -225,10 +225,14 @@ def _ptr(x) -> int:
     """Device/host address of a torch tensor, numpy array, or a plain int address."""
     if x is None:
         return 0
+    if type(x) is int:
+        return x
+    try:
+        return x.data_ptr()  # the usual case first: a call takes about ten of these
+    except AttributeError:
+        pass
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)!r}")
