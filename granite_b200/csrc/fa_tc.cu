@@ -163,7 +163,7 @@ struct TcSmem {
     int abort_flag;
     Item items[kMaxCachedItems];  // item of round r, worked out once at start-up instead of by every role at every item boundary
 };
-static_assert(sizeof(TcSmem<TcWindowItem>) <= 3072, "the barriers must fit beside seven 32 KB tiles");
+static_assert(sizeof(TcSmem<TcWindowItem>) <= 3 * 1024, "the barriers must fit beside seven 32 KB tiles");
 
 
 // fp32 -> fp16 hi + fp16 lo (x ~= hi + lo to about 22 bits), so fp32 queries lose nothing.

@@ -689,7 +689,7 @@ def test_structures_match_the_header(tmp_path):
 
 
 def test_reference_encoding_is_the_format():
-    """The checker's own e4m3 rounding, on every value, every midpoint and beyond the range; torch's cast as a second opinion."""
+    """The tests' own e4m3 rounding, on every value, every midpoint and beyond the range; torch's cast as a second opinion."""
     import torch
     v = R.e4m3_values()
     fine = np.isfinite(v)
