@@ -780,12 +780,12 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 #pragma unroll
                             for (int i = 0; i < 8; i++) {
                                 if constexpr (kQ8) {
-                                    // a page is two of the thread's column pairs; its scale is positive
+                                    // a page is two of the thread's column pairs; its K scale is positive
                                     if (i & 1) continue;
                                     const float pm = fmaxf(max3(__uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1]),
                                                                 __uint_as_float(x[h][4 * i + 4 + 2 * q])),
                                                            __uint_as_float(x[h][4 * i + 4 + 2 * q + 1]));
-                                    mm[h] = fmaxf(mm[h], pm * page_k[4 * h + i / 2]);
+                                    mm[h] = fmaxf(mm[h], fmaf(pm, page_k[4 * h + i / 2], page_lv[4 * h + i / 2]));
                                 } else {
                                     mm[h] = max3(mm[h], __uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1]));
                                 }
@@ -1299,9 +1299,12 @@ __global__ void __launch_bounds__(256) q8_gather_kernel(const __grid_constant__ 
                     v = p.v_scales[(size_t)e * p.hkv + h];
                 }
             }
-            // scale 0 comes with zero codes, so any positive number stands for it; 2^-60 of the largest V scale is beyond fp32 sums
+            // Scale 0 comes with zero codes, so any positive number stands for it.  V scales count as 2^-100 of the call's
+            // largest at least: a page of tiny values may hold most of a row's weight, and that weight is counted through its
+            // product 2^(s k scale - m) r.  m is at most the row's largest score, so the product of the page with that score is at
+            // least 2^-100, a normal number, and no weight passes 2^108.
             k = fmaxf(k, 1e-30f);
-            const float r = fmaxf(__fdiv_rn(v, m), 8.67361738e-19f);
+            const float r = fmaxf(__fdiv_rn(v, m), 7.88860905e-31f);
             const size_t at = (size_t)h * p.page_stride + page;
             p.page_k[at] = k * p.scale_log2;
             p.page_lv[at] = log2f(r);

@@ -1,0 +1,100 @@
+"""How exact attention over the 8-bit cache stays where magnitudes are spread: V scales that differ by many powers of two
+between pages, with the weight on the pages of small values or with the large ones closed to a row, and small queries
+against large keys.  Errors are held to each output's own sum of weight * |value|, not to the largest value of the call."""
+import numpy as np
+import pytest
+
+import view_reference as R
+from test_q8_cache import _dev, _table
+
+DEV = "cuda:0"
+
+
+def weighted_reference(q, codes, scales, v_codes, v_scales, pos, scale, cache_dtype, table, block_size=16, window=0, sinks=0):
+    """64-bit attention of q [R, Hq, D] at positions pos, and the bound on the error of each output.  With w the weights (largest
+    1), W their sum and A = sum w |v| / W:
+      * a weight is off by (D + 8) 2^-24 S (its fp32 score, S = sum |q k| scale; Q as fp16 hi + lo under a power of two is within
+        2^-22 of a head's largest element and counts there), by 2^-21 (exponential, hi + lo form), and by 2^-24 of the base-2 logarithms
+        of the V scales' ratio and of the score, which are added in fp32: relative errors, each at most twice into the mean;
+      * sums over n keys add n 2^-23 of A;
+      * a product of weight and V scale is held as fp16 hi + lo, to 2^-25 where it is small, in units in which the row's largest
+        product is at least 1/4: 2^-23 qmax max(w vs) / W for each key."""
+    rows, hq, d = q.shape
+    n = int(max(pos)) + 1
+    kv, vv = (R.rows_of(R.pool_values(c, s, cache_dtype, block_size), table, n, block_size) for c, s in ((codes, scales), (v_codes, v_scales)))
+    at = table[np.arange(n) // block_size]
+    seen = R.visible(pos, n, window, sinks)
+    want, bound, mean = np.zeros((rows, hq, d)), np.zeros((rows, hq, d)), np.zeros((rows, hq, d))
+    for h in range(hq):
+        g = h // (hq // kv.shape[1])
+        x = np.where(seen, (q[:, h] @ kv[:, g].T) * scale, -np.inf)
+        big = np.where(seen, (np.abs(q[:, h]).max(1, keepdims=True) * np.abs(kv[:, g]).sum(1)[None]) * scale, 0).max(1, keepdims=True)
+        top = x.max(1, keepdims=True)
+        w = np.exp(x - top)
+        total = w.sum(1, keepdims=True)
+        vs = v_scales[at, g].astype(np.float64)
+        live = vs[np.any(seen & (w > 0), 0)]
+        spread = np.log2(live.max() / live[live > 0].min()) if (live > 0).any() else 0.0
+        want[:, h] = w @ vv[:, g] / total
+        mean[:, h] = w @ np.abs(vv[:, g]) / total
+        rel = (d + 8) * 2.0 ** -24 * big + 2.0 ** -21 + 2.0 ** -24 * (spread + np.abs(top) * 1.443)
+        floor = n * 2.0 ** -23 * R.QMAX[cache_dtype] * (w * vs[None]).max(1, keepdims=True) / total
+        bound[:, h] = (2 * rel + n * 2.0 ** -23) * mean[:, h] + floor
+    return want, bound, mean
+
+
+def check(got, want, bound, mean, what):
+    got = np.asarray(got, np.float64)
+    assert np.isfinite(got).all(), what
+    over = np.abs(got - want) - bound
+    assert over.max() <= 0, f"{what}: off by {np.abs(got - want).max():.3e}, {over.max():.3e} over the bound"
+    # per (row, head): errors of sums of at most 2^15 terms add up like a random walk
+    rel = np.linalg.norm(got - want, axis=-1) / np.linalg.norm(mean, axis=-1)
+    assert rel.max() <= 2.0 ** -16.5, f"{what}: {rel.max():.3e} of the weighted values at {np.unravel_index(rel.argmax(), rel.shape)}"
+
+
+def spread_pools(rng, blocks, hkv, d, cache_dtype, table, n, q_dir, scale, v_log2, tilt):
+    """Pools whose page scales of V are 2^v_log2[page] and whose keys give a token of logical page p the score
+    -tilt * ln(V scale) + noise against q_dir [Hkv, D]: with tilt above 1 the weight sits on the pages of small values."""
+    kc = np.zeros((blocks * 16, hkv, d), np.uint8)
+    ks = np.ones((blocks, hkv), np.float32)
+    vc, vs = R.random_pool(rng, blocks, 16, hkv, d, cache_dtype)
+    vc, vs = vc.copy(), vs.copy()
+    for p in range((n + 15) // 16):
+        e = table[p]
+        vs[e] = (vs[e] * 2.0 ** v_log2[p]).astype(np.float32)
+        target = -tilt * np.log(vs[e].astype(np.float64))[None, :] + rng.standard_normal((16, hkv))
+        k = target[..., None] * q_dir / ((q_dir ** 2).sum(-1, keepdims=True) * scale) + 0.05 * rng.standard_normal((16, hkv, d))
+        ks[e] = (np.abs(k).max((0, 2)) / R.QMAX[cache_dtype]).astype(np.float32)
+        kc[e * 16:e * 16 + 16] = R.encode(k / ks[e][None, :, None], cache_dtype)
+    return kc, ks, vc, vs
+
+
+PREFILLS = [(300, 0, 8, 2, 128), (140, 333, 4, 1, 64), (40, 1200, 4, 2, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", [0, 1])
+@pytest.mark.parametrize("seq,start,hq,hkv,d", PREFILLS)
+@pytest.mark.parametrize("bits,tilt,order", [(12, 0.0, "later"), (24, 0.0, "later"), (40, 0.0, "later"), (20, 1.5, "mixed"), (30, 1.2, "earlier")])
+def test_prefill_q8_with_spread_v_scales(compute, cache_dtype, seq, start, hq, hkv, d, bits, tilt, order):
+    """`later`: V grows by 2^bits towards the chunk's end, so that early rows may not see the large pages; otherwise the weight sits
+    on pages of small values."""
+    import torch
+    rng = np.random.default_rng(bits + seq + d)
+    n, scale = start + seq, d ** -0.5
+    tables, blocks = _table(rng, [n], 16)
+    pages = (n + 15) // 16
+    v_log2 = np.linspace(-bits, 0, pages)
+    if order == "earlier":
+        v_log2 = v_log2[::-1]
+    if order == "mixed":
+        v_log2 = rng.permutation(v_log2)
+    q_dir = rng.standard_normal((hkv, d))
+    q = (np.repeat(q_dir, hq // hkv, 0)[None] * (1 + 0.02 * rng.standard_normal((seq, hq, 1)))).astype(np.float32)
+    kc, ks, vc, vs = spread_pools(rng, blocks, hkv, d, cache_dtype, tables[0], n, q_dir, scale, v_log2, tilt)
+    ref = weighted_reference(q.astype(np.float64), kc, ks, vc, vs, start + np.arange(seq), scale, cache_dtype, tables[0])
+    out = torch.full(q.shape, float("nan"), device=DEV)
+    compute.paged_prefill_attention_q8(*[_dev(x) for x in (q, kc, vc, ks, vs, tables)], out, hq, hkv, seq, start, d, 16, tables.shape[1], blocks, scale, cache_dtype)
+    compute.sync()
+    check(out.cpu().numpy(), *ref, f"{seq}@{start} 2^{bits} {order}")
