@@ -33,9 +33,10 @@
 // its token per 16-dim unit, and Q is loaded in that order; for V (transposed) it gets two neighbouring dims of two tokens,
 // which are two rows of the output tile.  Code pairs become fp16 pairs in registers, exactly (int8 scores need not: they
 // are integer products with the digits of Q).  A page's K scale
-// multiplies its fp32 scores; its V scale multiplies the weights, relative to a power of two that follows the largest V scale
-// seen (so weights stay bounded), and that power multiplies the accumulators at the end.  The scales of 32 pages are
-// loaded at a time, one page per lane, one batch ahead of use.
+// multiplies its fp32 scores; its V scale multiplies the weights, whose products are held relative to a power of two per query head
+// that follows the largest product met so far.  (That keeps the largest products near 1, where fp16 hi + lo has 22 bits.  A power that
+// follows the largest V scale does not: a page of large values and no weight to speak of took the other pages' bits - 5e-3 off
+// for V scales of 2^-16 of the largest.)  The scales of 32 pages are loaded at a time, one page per lane, one batch ahead of use.
 //
 // Sliding window (kWindow).  A sequence is walked as the list of its visible pages - sink pages, then the window's - so
 // the work is planned and balanced over those alone; the two pages at the list's inner edges are masked by token.
@@ -867,7 +868,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
             // One page per iteration; with split pages a warp's are every page_split-th, by their place in the ring.
             const int step = split ? p.page_split : 1;
             const int first = split ? (sub - (slot >> 1)) & (step - 1) : 0;
-            int v_exp = -126;  // the weights carry V scales relative to 2^v_exp
+            // Products of weight and V scale are held times `unit`, a power of two, and so are the sums of products; weights
+            // themselves, and their sum, are relative to 2^m_run alone.
+            float unit[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) unit[nt][0] = unit[nt][1] = 1.f;
             int at = slot + 2 * first;  // slot of K of page j (V is the slot after it) and its parity
             uint32_t ph = phase;
             if (at >= p.slots) {
@@ -904,23 +909,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                         scales_of(sb.entry, sb.k_next, sb.v_next);
                         sb.entry = page_entry((j & ~31) + 64 + lane);
                     }
-                    // the smallest power of two that no V scale of these pages exceeds; growing it rescales what is summed
-                    int e = (int)((__float_as_uint(sb.v) >> 23) & 0xFF) - 126;
-#pragma unroll
-                    for (int sh = 16; sh > 0; sh >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, sh));
-                    if (e > v_exp) {
-                        const float f = exp2f((float)(v_exp - e));
-                        v_exp = e;
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int mt = 0; mt < kDSteps; mt++)
-#pragma unroll
-                                for (int i = 0; i < 4; i++) o[nt][mt][i] *= f;
-                    }
-                    sb.v *= exp2f((float)-v_exp);
                 }
-                const float k_scale = __shfl_sync(0xffffffffu, sb.k, j & 31), v_weight = __shfl_sync(0xffffffffu, sb.v, j & 31);
+                const float k_scale = __shfl_sync(0xffffffffu, sb.k, j & 31), v_scale = __shfl_sync(0xffffffffu, sb.v, j & 31);
 
                 // ---- S^T = K Q^T, two 16-dim units per ldmatrix, independent MMA chains
                 float s0[NT][4] = {}, s1[NT][4] = {};
@@ -953,9 +943,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                 }
                 release(at_k);
 
-                // ---- scores less the running maximum (in log2 units).  The maximum is only raised when a score passes it by
-                // 2^8: weights stay below 256, and the usual page costs one vote instead of a reduction.
+                // ---- scores less the running maximum (in log2 units).  The maximum is only raised when a weight, or its product with
+                // the V scale in units, would pass 2^8: both stay below 256, and the usual page costs one vote instead of a reduction.
                 float x[NT][4];
+                float limit[NT][2];  // for a score
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        // v_scale unit < 2^u: the exponents added (the unit's mantissa is zero), both of them biased
+                        const int u = (int)((__float_as_uint(v_scale) + __float_as_uint(unit[nt][c])) >> 23) - 253;
+                        limit[nt][c] = m_run[nt][c] + 8.f - (float)max(u, 0);
+                    }
                 bool grow = false;
                 const bool seen0 = (rows >> g) & 1u, seen1 = (rows >> (g + 8)) & 1u;
 #pragma unroll
@@ -973,7 +972,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                         if (kPair) v += __shfl_xor_sync(0xffffffffu, v, 2);
                         if constexpr (kElem == kElemInt8) v *= q_step[nt][i & 1];
                         x[nt][i] = (i < 2 ? seen0 : seen1) ? v * k_scale : -INFINITY;
-                        grow |= x[nt][i] > m_run[nt][i & 1] + 8.f;
+                        grow |= x[nt][i] > limit[nt][i & 1];
                     }
                 }
                 if (__any_sync(0xffffffffu, grow)) {
@@ -985,10 +984,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                             float m = fmaxf(x[nt][c], x[nt][2 + c]);
 #pragma unroll
                             for (int sh = 4; sh < 32; sh <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
-                            m = fmaxf(m, m_run[nt][c]);
-                            a01[c] = fast_exp2(m_run[nt][c] - m);
-                            m_run[nt][c] = m;
-                            l_run[nt][c] *= a01[c];
+                            const float m_old = m_run[nt][c], m_new = fmaxf(m, m_old);
+                            // the largest products, in log2: so far, and at most, of this page
+                            const float d_old = (float)((int)(__float_as_uint(unit[nt][c]) >> 23) - 127);
+                            const float v_log2 = (float)((int)(__float_as_uint(v_scale) >> 23) - 126);
+                            const float d = fminf(fmaxf(floorf(m_new - fmaxf(m_old - d_old, m + v_log2)), -126.f), 120.f);
+                            m_run[nt][c] = m_new;
+                            unit[nt][c] = __int_as_float(((int)d + 127) << 23);
+                            l_run[nt][c] *= fast_exp2(m_old - m_new);
+                            a01[c] = fast_exp2(m_old - m_new + (d - d_old));
                         }
 #pragma unroll
                         for (int mt = 0; mt < kDSteps; mt++)
@@ -1004,9 +1008,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                     for (int i = 0; i < 4; i++) w[i] = fast_exp2(x[nt][i] - m_run[nt][i & 1]);
                     l_run[nt][0] += w[0] + w[2];
                     l_run[nt][1] += w[1] + w[3];
+                    float f0 = v_scale * unit[nt][0], f1 = v_scale * unit[nt][1];
+                    if (f0 > 0x1p126f) f0 = 0x1p126f;  // (infinite only where the weights are zero; a NaN stays)
+                    if (f1 > 0x1p126f) f1 = 0x1p126f;
 #pragma unroll
                     for (int half = 0; half < 2; half++) {
-                        const float w0 = w[2 * half] * v_weight, w1 = w[2 * half + 1] * v_weight;
+                        const float w0 = w[2 * half] * f0, w1 = w[2 * half + 1] * f1;
                         const __half2 h = __floats2half2_rn(w0, w1);
                         const float2 back = __half22float2(h);
                         const __half2 l = __floats2half2_rn(w0 - back.x, w1 - back.y);
@@ -1059,13 +1066,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
             slot += 2 * seg.npages;
             phase ^= (uint32_t)(slot / p.slots) & 1u;
             slot %= p.slots;
-            const float f = exp2f((float)v_exp);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < NT; nt++) {
+                const float f[2] = {1.f / unit[nt][0], 1.f / unit[nt][1]};
 #pragma unroll
                 for (int mt = 0; mt < kDSteps; mt++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) o[nt][mt][i] *= f;
+                    for (int i = 0; i < 4; i++) o[nt][mt][i] *= f[i & 1];
+            }
         } else
         // PP pages per iteration.  With head_dim 64 a page is half the bytes for the same chain of
         // waits, shuffles and exponentials, so two pages share one softmax round (32 tokens) and

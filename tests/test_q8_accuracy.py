@@ -98,3 +98,43 @@ def test_prefill_q8_with_spread_v_scales(compute, cache_dtype, seq, start, hq, h
     compute.paged_prefill_attention_q8(*[_dev(x) for x in (q, kc, vc, ks, vs, tables)], out, hq, hkv, seq, start, d, 16, tables.shape[1], blocks, scale, cache_dtype)
     compute.sync()
     check(out.cpu().numpy(), *ref, f"{seq}@{start} 2^{bits} {order}")
+
+
+DECODES = [(8, 2, 128, [1000, 64, 333, 17]), (32, 8, 128, [2100, 700] * 12), (8, 1, 64, [900, 40]), (16, 2, 128, [3000, 500] * 40), (10, 2, 128, [777, 50]), (24, 2, 64, [600] * 3),
+           (12, 1, 128, [500])]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", [0, 1])
+@pytest.mark.parametrize("hq,hkv,d,lens", DECODES)
+@pytest.mark.parametrize("bits,tilt", [(12, 1.3), (20, 1.5), (30, 1.2), (60, 1.4)])
+def test_decode_q8_with_spread_v_scales(compute, cache_dtype, hq, hkv, d, lens, bits, tilt):
+    """The weight sits on pages of small values, pages of large values have next to none: one sequence and many, cut between
+    CTAs and warps and not."""
+    import torch
+    rng = np.random.default_rng(bits + hq + d)
+    scale = d ** -0.5
+    lens = np.asarray(lens, np.int32)
+    kinds = {}  # sequences of one length share their pages, so that the reference is worked out once for each
+    parts, tables, blocks = [], np.full((len(lens), (lens.max() + 15) // 16), -1, np.int32), 0
+    q_dir = rng.standard_normal((hkv, d))
+    q1 = (np.repeat(q_dir, hq // hkv, 0) * (1 + 0.02 * rng.standard_normal((hq, 1)))).astype(np.float32)
+    for b, n in enumerate(lens):
+        if n not in kinds:
+            t, count = _table(rng, [n], 16)
+            pages = (n + 15) // 16
+            pools = spread_pools(rng, count, hkv, d, cache_dtype, t[0], n, q_dir, scale, rng.uniform(-bits, 0, pages), tilt)
+            kinds[n] = (blocks, t[0], weighted_reference(q1[None].astype(np.float64), *pools, [n - 1], scale, cache_dtype, t[0]))
+            parts.append(pools)
+            blocks += count
+        base, t, _ = kinds[n]
+        tables[b, :len(t)] = t + base
+    kc, ks, vc, vs = (np.concatenate(x) for x in zip(*parts))
+    q = np.broadcast_to(q1, (len(lens), hq, d)).copy()
+    out = torch.full(q.shape, float("nan"), device=DEV)
+    compute.batched_paged_attention_decode_q8(*[_dev(x) for x in (q, kc, vc, ks, vs, tables, lens)], out, len(lens), hq, hkv, d, 16, tables.shape[1], scale,
+                                              num_blocks=blocks, cache_dtype=cache_dtype)
+    compute.sync()
+    got = out.cpu().numpy()
+    for b, n in enumerate(lens):
+        check(got[b:b + 1], *kinds[n][2], f"sequence {b} of {n}, 2^{bits}")
