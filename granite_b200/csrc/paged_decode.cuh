@@ -541,6 +541,31 @@ __device__ __forceinline__ void q8_pairs(uint32_t w, uint32_t& lo, uint32_t& hi)
 // |i| < 2^22, exactly: added to the bits of 1.5 * 2^23 it is that number plus i.
 __device__ __forceinline__ float small_int_to_float(int i) { return __int_as_float(0x4B400000 + i) - 12582912.f; }
 
+// A power of two for each score column of a lane (two per n-tile), kept by its biased exponent (1 to 254): as the numbers
+// themselves for up to four query heads per warp, packed into one register above that, where registers are short (64 sequences of up
+// to 32768 tokens in e4m3: 16 query heads per KV head 1128 us packed against 1375, 8 heads 426 against 450; four heads in int8 the
+// other way round, 363 against 358).
+template <bool kPacked>
+struct ColumnPow2 {
+    float value[2];
+    __device__ float get(int, int c) const { return value[c]; }
+    __device__ int exponent(int, int c) const { return (int)(__float_as_uint(value[c]) >> 23); }
+    __device__ void set(int, int c, int biased) { value[c] = __int_as_float(biased << 23); }
+};
+template <>
+struct ColumnPow2<true> {
+    uint32_t packed;  // byte 2 nt + c
+    __device__ float get(int nt, int c) const {
+        const int i = 2 * nt + c;
+        return __uint_as_float((i < 3 ? packed << (23 - 8 * i) : packed >> 1) & 0x7F800000u);
+    }
+    __device__ int exponent(int nt, int c) const { return (int)((packed >> (8 * (2 * nt + c))) & 0xFFu); }
+    __device__ void set(int nt, int c, int biased) {
+        const int at = 8 * (2 * nt + c);
+        packed = (packed & ~(0xFFu << at)) | ((uint32_t)biased << at);
+    }
+};
+
 // The scales of up to 32 listed pages, one per lane, and the entries of the batch after them: the chain table entry ->
 // scale is two trips to memory, so entries are fetched two batches ahead and scales one.
 struct ScaleBatch {
@@ -778,7 +803,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
         // d0 | d1 of four heads and d2 | nothing.
         constexpr int kDigitTiles = kPair ? 2 : 3 * NT;
         uint32_t qd[kElem == kElemInt8 ? kDigitTiles : 1][kDSteps / 2][2];
-        float q_step[NT][2];  // of the heads of the lane's score columns
+        float q_step[NT][2];  // int8: what Q of the heads of the lane's score columns is held in units of
+        ColumnPow2<!kPair> q_pow2{};  // e4m3: the same
         if constexpr (kElem == kElemInt8) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -835,6 +861,24 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
             const int n = kPair ? (g & 3) : nt * 8 + g;
             const bool valid = n < n_q;
             const float* qp = p.q + ((size_t)seg.seq * p.num_heads + hq0 + (valid ? n : 0)) * D;
+            // e4m3: a power of two per head brings the largest |q| into [2^14, 2^15), so that hi + lo has 22 bits of every element down
+            // to 2^-14 of it, whatever the magnitude (small queries may meet keys with large scales)
+            float q_scale = p.scale_log2;
+            if constexpr (kElem == kElemE4M3) {
+                float big = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < kDSteps; ks++) {
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (valid) v = *reinterpret_cast<const float4*>(qp + ks * 16 + 4 * t);
+                    big = fmaxf(fmaxf(big, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                }
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -112), 127);
+                q_scale = __int_as_float((14 - e + 127) << 23);
+#pragma unroll
+                for (int c = 0; c < 2; c++) q_pow2.set(nt, c, __shfl_sync(0xffffffffu, e - 14 + 127, (kPair ? (2 * t + c) & 3 : 2 * t + c) * 4));
+            }
 #pragma unroll
             for (int ks = 0; ks < kDSteps; ks++) {
 #pragma unroll
@@ -842,8 +886,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                     float2 v = make_float2(0.f, 0.f);
                     const int dim = ks * 16 + (kElem == kElemF16 ? half * 8 + 2 * t : 4 * t + half * 2);
                     if (valid) v = *reinterpret_cast<const float2*>(qp + dim);
-                    v.x *= p.scale_log2;
-                    v.y *= p.scale_log2;
+                    v.x *= q_scale;
+                    v.y *= q_scale;
                     __half2 hi = __floats2half2_rn(v.x, v.y);
                     float2 back = __half22float2(hi);
                     __half2 lo = __floats2half2_rn(v.x - back.x, v.y - back.y);
@@ -868,11 +912,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
             // One page per iteration; with split pages a warp's are every page_split-th, by their place in the ring.
             const int step = split ? p.page_split : 1;
             const int first = split ? (sub - (slot >> 1)) & (step - 1) : 0;
-            // Products of weight and V scale are held times `unit`, a power of two, and so are the sums of products; weights
-            // themselves, and their sum, are relative to 2^m_run alone.
-            float unit[NT][2];
+            // Products of weight and V scale are held times a power of two, and so are the sums of products; weights themselves,
+            // and their sum, are relative to 2^m_run alone.
+            ColumnPow2<!kPair> unit{};
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) unit[nt][0] = unit[nt][1] = 1.f;
+            for (int nt = 0; nt < NT; nt++) unit.set(nt, 0, 127), unit.set(nt, 1, 127);
             int at = slot + 2 * first;  // slot of K of page j (V is the slot after it) and its parity
             uint32_t ph = phase;
             if (at >= p.slots) {
@@ -947,13 +991,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                 // the V scale in units, would pass 2^8: both stay below 256, and the usual page costs one vote instead of a reduction.
                 float x[NT][4];
                 float limit[NT][2];  // for a score
+                float ks[NT][2];     // what a sum of products is multiplied by
+                const float k_log2 = kElem == kElemE4M3 ? k_scale * p.scale_log2 : k_scale;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        // v_scale unit < 2^u: the exponents added (the unit's mantissa is zero), both of them biased
-                        const int u = (int)((__float_as_uint(v_scale) + __float_as_uint(unit[nt][c])) >> 23) - 253;
+                        // v_scale unit < 2^u: the exponents added, both of them biased
+                        const int u = (int)(__float_as_uint(v_scale) >> 23) + unit.exponent(nt, c) - 253;
                         limit[nt][c] = m_run[nt][c] + 8.f - (float)max(u, 0);
+                        ks[nt][c] = kElem == kElemE4M3 ? k_log2 * q_pow2.get(nt, c) : k_scale;
                     }
                 bool grow = false;
                 const bool seen0 = (rows >> g) & 1u, seen1 = (rows >> (g + 8)) & 1u;
@@ -971,7 +1018,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                         }
                         if (kPair) v += __shfl_xor_sync(0xffffffffu, v, 2);
                         if constexpr (kElem == kElemInt8) v *= q_step[nt][i & 1];
-                        x[nt][i] = (i < 2 ? seen0 : seen1) ? v * k_scale : -INFINITY;
+                        x[nt][i] = (i < 2 ? seen0 : seen1) ? v * ks[nt][i & 1] : -INFINITY;
                         grow |= x[nt][i] > limit[nt][i & 1];
                     }
                 }
@@ -986,11 +1033,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                             for (int sh = 4; sh < 32; sh <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
                             const float m_old = m_run[nt][c], m_new = fmaxf(m, m_old);
                             // the largest products, in log2: so far, and at most, of this page
-                            const float d_old = (float)((int)(__float_as_uint(unit[nt][c]) >> 23) - 127);
+                            const float d_old = (float)(unit.exponent(nt, c) - 127);
                             const float v_log2 = (float)((int)(__float_as_uint(v_scale) >> 23) - 126);
                             const float d = fminf(fmaxf(floorf(m_new - fmaxf(m_old - d_old, m + v_log2)), -126.f), 120.f);
                             m_run[nt][c] = m_new;
-                            unit[nt][c] = __int_as_float(((int)d + 127) << 23);
+                            unit.set(nt, c, (int)d + 127);
                             l_run[nt][c] *= fast_exp2(m_old - m_new);
                             a01[c] = fast_exp2(m_old - m_new + (d - d_old));
                         }
@@ -1008,7 +1055,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                     for (int i = 0; i < 4; i++) w[i] = fast_exp2(x[nt][i] - m_run[nt][i & 1]);
                     l_run[nt][0] += w[0] + w[2];
                     l_run[nt][1] += w[1] + w[3];
-                    float f0 = v_scale * unit[nt][0], f1 = v_scale * unit[nt][1];
+                    float f0 = v_scale * unit.get(nt, 0), f1 = v_scale * unit.get(nt, 1);
                     if (f0 > 0x1p126f) f0 = 0x1p126f;  // (infinite only where the weights are zero; a NaN stays)
                     if (f1 > 0x1p126f) f1 = 0x1p126f;
 #pragma unroll
@@ -1068,7 +1115,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
             slot %= p.slots;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const float f[2] = {1.f / unit[nt][0], 1.f / unit[nt][1]};
+                const float f[2] = {1.f / unit.get(nt, 0), 1.f / unit.get(nt, 1)};
 #pragma unroll
                 for (int mt = 0; mt < kDSteps; mt++)
 #pragma unroll

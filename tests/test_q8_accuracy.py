@@ -138,3 +138,30 @@ def test_decode_q8_with_spread_v_scales(compute, cache_dtype, hq, hkv, d, lens, 
     got = out.cpu().numpy()
     for b, n in enumerate(lens):
         check(got[b:b + 1], *kinds[n][2], f"sequence {b} of {n}, 2^{bits}")
+
+
+def small_query_case(rng, n, rows, hq, hkv, d, cache_dtype, magnitude):
+    """Queries of the given magnitude (with one element of every head much larger than the others in half of the heads) over keys
+    whose scales make up for it."""
+    t, blocks = _table(rng, [n], 16)
+    (kc, ks), (vc, vs) = (R.random_pool(rng, blocks, 16, hkv, d, cache_dtype) for _ in range(2))
+    q = (rng.standard_normal((rows, hq, d)) * magnitude).astype(np.float32)
+    q[:, ::2, 3] *= 30
+    return t, blocks, q, kc, (ks / np.float32(magnitude)).astype(np.float32), vc, vs
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", [0, 1])
+@pytest.mark.parametrize("hq,hkv,d,n", [(8, 2, 128, 700), (32, 4, 64, 100), (16, 1, 128, 1500)])
+@pytest.mark.parametrize("magnitude", [1e-2, 1e-4, 1e-9, 1e-20, 1e6])
+def test_decode_q8_queries_of_any_magnitude(compute, cache_dtype, hq, hkv, d, n, magnitude):
+    """q . k is the same product whichever of the two holds the magnitude."""
+    import torch
+    rng = np.random.default_rng(n)
+    t, blocks, q, kc, ks, vc, vs = small_query_case(rng, n, 1, hq, hkv, d, cache_dtype, magnitude)
+    ref = weighted_reference(q.astype(np.float64), kc, ks, vc, vs, [n - 1], d ** -0.5, cache_dtype, t[0])
+    out = torch.full(q.shape, float("nan"), device=DEV)
+    compute.batched_paged_attention_decode_q8(*[_dev(x) for x in (q, kc, vc, ks, vs, t)], _dev(np.array([n], np.int32)), out, 1, hq, hkv, d, 16, t.shape[1],
+                                              d ** -0.5, num_blocks=blocks, cache_dtype=cache_dtype)
+    compute.sync()
+    check(out.cpu().numpy(), *ref, f"{magnitude}")
