@@ -96,6 +96,7 @@ struct TcParams {
     const float* page_iv;
     const float* v_max;
     int page_stride;
+    const float* q_step;        // kQ8 with fp32 queries: [row, head], what a score is multiplied by besides
     // kWindow: pieces that every item's tiles are cut into; with more than one, [row, head, chunk] partials
     int n_chunks;
     float* part_o;
@@ -184,7 +185,38 @@ __global__ void split_f32_to_f16_kernel(const float4* __restrict__ src, uint4* _
     hi[i] = make_uint4(h[0], h[1], h[2], h[3]);
     lo[i] = make_uint4(l[0], l[1], l[2], l[3]);
 }
-// The same for a source that is not 16-byte aligned.
+// The same for the 8-bit cache, under a power of two per row and head that brings the largest |q| into [2^14, 2^15): hi + lo then has
+// 22 bits of every element down to 2^-14 of it, whatever the magnitude (small queries may meet keys with large scales).
+// `step` [rows, heads] takes what the scores are to be multiplied by.  kD: head_dim; kD / 8 neighbouring threads hold a head.
+template <int kD>
+__global__ void split_f32_to_f16_scaled_kernel(const float4* __restrict__ src, uint4* __restrict__ hi, uint4* __restrict__ lo,
+                                               float* __restrict__ step, size_t n8) {
+    const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const bool here = i < n8;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 a = here ? src[2 * i] : zero, b = here ? src[2 * i + 1] : zero;
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    float big = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) big = fmaxf(big, fabsf(x[k]));
+#pragma unroll
+    for (int sh = kD / 16; sh > 0; sh >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, sh));
+    const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -112), 127);
+    const float scale = __int_as_float((14 - e + 127) << 23);
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float y0 = x[2 * k] * scale, y1 = x[2 * k + 1] * scale;
+        h[k] = pack_half2(y0, y1);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h[k]));
+        l[k] = pack_half2(y0 - back.x, y1 - back.y);
+    }
+    if (!here) return;
+    hi[i] = make_uint4(h[0], h[1], h[2], h[3]);
+    lo[i] = make_uint4(l[0], l[1], l[2], l[3]);
+    if (i % (kD / 8) == 0) step[i / (kD / 8)] = __int_as_float((e - 14 + 127) << 23);
+}
+// The first for a source that is not 16-byte aligned.
 __global__ void split_f32_to_f16_single_kernel(const float* __restrict__ src, __half* __restrict__ hi,
                                                __half* __restrict__ lo, size_t n) {
     const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -685,6 +717,12 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     anc[q] = ancestor_word(par, node, N) >> (2 * tq);
                 }
             }
+            float q_step[2] = {1.f, 1.f};
+            if constexpr (kQ8 && kSplitQ) {
+#pragma unroll
+                for (int q = 0; q < 2; q++)
+                    if (row_of[q] < it.rows_here) q_step[q] = __ldg(p.q_step + (size_t)(it.q0 + row_of[q]) * p.num_heads + it.head0);
+            }
             float m_used_t[kTiles][2], l_run_t[kTiles][2];  // running maximum and (per-thread part of the) sum, per tile and row
             const int o_sel = kDefer ? (items_done & 1) : 0;  // accumulator of this item (see the output MMAs)
             {
@@ -785,7 +823,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                                     const float pm = fmaxf(max3(__uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1]),
                                                                 __uint_as_float(x[h][4 * i + 4 + 2 * q])),
                                                            __uint_as_float(x[h][4 * i + 4 + 2 * q + 1]));
-                                    mm[h] = fmaxf(mm[h], fmaf(pm, page_k[4 * h + i / 2], page_lv[4 * h + i / 2]));
+                                    mm[h] = fmaxf(mm[h], fmaf(pm, kSplitQ ? page_k[4 * h + i / 2] * q_step[q] : page_k[4 * h + i / 2], page_lv[4 * h + i / 2]));
                                 } else {
                                     mm[h] = max3(mm[h], __uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1]));
                                 }
@@ -842,9 +880,11 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
 #pragma unroll
                             for (int pg = 0; pg < 4; pg++) {
                                 const float iv = page_iv[4 * h + pg];
-                                const uint64_t iv2 = f32x2(iv, iv), k2 = f32x2(page_k[4 * h + pg], page_k[4 * h + pg]);
+                                const uint64_t iv2 = f32x2(iv, iv);
 #pragma unroll
                                 for (int q = 0; q < 2; q++) {
+                                    const float k = kSplitQ ? page_k[4 * h + pg] * q_step[q] : page_k[4 * h + pg];
+                                    const uint64_t k2 = f32x2(k, k);
                                     // 2^(s k - m + log2(v / v_max)); masked scores are -inf and give exactly 0
                                     const float off = page_lv[4 * h + pg] - m_used[q];
                                     const uint64_t off2 = f32x2(off, off);
@@ -1395,15 +1435,27 @@ int launch_paged_prefill_q8(granite_cuda_compute* c, const GraniteCudaPagedPrefi
         g.skip = first - g.head_pages;
     }
     const size_t n_q = (size_t)a.seq_q * a.num_heads * D;
-    const size_t q_bytes = split_q ? split_bytes(n_q) : 0;
+    const size_t step_bytes = (n_q / D * sizeof(float) + 255) / 256 * 256;
+    const size_t q_bytes = split_q ? split_bytes(n_q) + step_bytes : 0;
     const size_t kv_bytes = (size_t)g.hkv * g.rows * D * 2;                                           // a multiple of 128 rows * 128 bytes
     const size_t page_bytes = ((size_t)g.hkv * g.page_stride * 4 + 255) / 256 * 256;
     const size_t partials = plan_chunks(c, p, (int)D);
     const size_t fixed = 2 * kv_bytes + 3 * page_bytes + ((size_t)g.hkv * 4 + 255) / 256 * 256;
     const size_t behind = fixed + partials;
     const void *q16 = a.q, *q16_lo = a.q;
-    int rc = split_q ? split_queries(c, a.q, n_q, &q16, &q16_lo, behind) : c->ensure_scratch(behind);
+    int rc = c->ensure_scratch(q_bytes + behind);
     if (rc) return rc;
+    if (split_q) {
+        uint8_t* at = static_cast<uint8_t*>(c->scratch);
+        q16 = at;
+        q16_lo = at + split_bytes(n_q) / 2;
+        p.q_step = reinterpret_cast<float*>(at + split_bytes(n_q));
+        LaunchScope t(c, "split_q_f16");
+        auto kern = D == 128 ? split_f32_to_f16_scaled_kernel<128> : split_f32_to_f16_scaled_kernel<64>;
+        kern<<<(unsigned)((n_q / 8 + 255) / 256), 256, 0, c->stream>>>(static_cast<const float4*>(a.q), reinterpret_cast<uint4*>(at),
+                                                                     reinterpret_cast<uint4*>(at + split_bytes(n_q) / 2), const_cast<float*>(p.q_step), n_q / 8);
+        GB_CUDA_TRY(cudaGetLastError());
+    }
     uint8_t* ws = static_cast<uint8_t*>(c->scratch) + q_bytes;
     place_partials(p, ws + fixed, (int)D);
     g.k16 = reinterpret_cast<__half*>(ws);
