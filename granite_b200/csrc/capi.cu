@@ -55,13 +55,23 @@ int granite_cuda_compute::retire(void* old) {
     return GRANITE_CUDA_SUCCESS;
 }
 
+bool granite_cuda_compute::capturing() {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &st) != cudaSuccess) cudaGetLastError();
+    if (st != cudaStreamCaptureStatusNone) captured = true;
+    return st != cudaStreamCaptureStatusNone;
+}
+
+// Nothing grows during a capture, whatever its mode allows: work on a new allocation (clearing the counters) would become part of the
+// graph, while calls outside it would use the allocation at once.
+static int refuse_growth(const char* what) {
+    return fail(GRANITE_CUDA_INVALID_STATE, std::string(what) + " would have to grow while the stream is being captured: make the call once before the capture");
+}
+
 int granite_cuda_compute::ensure_scratch(size_t bytes) {
-    if (!captured) {
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(stream, &st) != cudaSuccess) cudaGetLastError();
-        captured = st == cudaStreamCaptureStatusActive;
-    }
+    if (!captured) capturing();
     if (bytes <= scratch_bytes) return GRANITE_CUDA_SUCCESS;
+    if (capturing()) return refuse_growth("scratch arena");
     size_t want = bytes + bytes / 4;
     void* grown = nullptr;
     if (cudaMalloc(&grown, want) != cudaSuccess) {
@@ -76,6 +86,7 @@ int granite_cuda_compute::ensure_scratch(size_t bytes) {
 
 int granite_cuda_compute::ensure_page_counters(size_t count) {
     if (count <= pages_done_count) return GRANITE_CUDA_SUCCESS;
+    if (capturing()) return refuse_growth("decode page counters");
     const size_t want = count + count / 4 + 1024;
     int* grown = nullptr;
     if (cudaMalloc(&grown, want * sizeof(int)) != cudaSuccess) {

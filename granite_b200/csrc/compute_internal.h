@@ -79,6 +79,7 @@ struct granite_cuda_compute {
     void* scratch = nullptr;
     size_t scratch_bytes = 0;
     bool captured = false;  // a call has been made while the stream was capturing
+    bool capturing();       // whether it is now (and notes that it was)
     std::vector<void*> retired;
     int retire(void* old);
     // Cached TMA descriptors, keyed by (buffer, shape).  Bounded: once kMaxTensorMaps entries exist,

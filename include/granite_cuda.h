@@ -46,7 +46,10 @@ enum {
 };
 
 /* Opaque compute object: one device, one stream, cached tensor maps and scratch memory.
- * Replaces the MetalCompute singleton (include/granite/metal_compute.h:20-66); one per GPU. */
+ * Replaces the MetalCompute singleton (include/granite/metal_compute.h:20-66); one per GPU.
+ * Scratch memory grows with the calls that need more of it.  It does not grow while the stream is being captured: such a
+ * call returns GRANITE_CUDA_INVALID_STATE and leaves the capture as it was (make the call once before).  A captured graph
+ * uses the object's scratch memory like a call: the object's calls and the replays of its graphs must not overlap. */
 typedef struct granite_cuda_compute granite_cuda_compute_t;
 
 /* Message of the last failing call on this thread (never NULL). */
