@@ -42,16 +42,23 @@ static EncodeTiledFn encode_tiled_fn() {
 
 using namespace gb200;
 
-// An allocation that is replaced by a larger one: freed once the calls in flight are done, or kept until the object goes when
-// a captured graph may hold it.
-int granite_cuda_compute::retire(void* old) {
-    if (!old) return GRANITE_CUDA_SUCCESS;
-    if (captured) {
-        retired.push_back(old);
-        return GRANITE_CUDA_SUCCESS;
+// Replaces an allocation by a larger one.  The old one is freed first, once the calls in flight are done, so that growing needs no more
+// than the new size; one that a captured graph may hold is kept until the object goes.
+int granite_cuda_compute::grow(void** held, size_t* count, size_t want, size_t unit, const char* what) {
+    if (*held && captured) {
+        retired.push_back(*held);
+    } else if (*held) {
+        GB_CUDA_TRY(cudaStreamSynchronize(stream));
+        GB_CUDA_TRY(cudaFree(*held));
     }
-    GB_CUDA_TRY(cudaStreamSynchronize(stream));
-    GB_CUDA_TRY(cudaFree(old));
+    *held = nullptr;
+    *count = 0;
+    if (cudaMalloc(held, want * unit) != cudaSuccess) {
+        cudaGetLastError();
+        *held = nullptr;
+        return fail(GRANITE_CUDA_OUT_OF_MEMORY, std::string(what) + ": cudaMalloc of " + std::to_string(want * unit) + " bytes failed");
+    }
+    *count = want;
     return GRANITE_CUDA_SUCCESS;
 }
 
@@ -72,36 +79,22 @@ int granite_cuda_compute::ensure_scratch(size_t bytes) {
     if (!captured) capturing();
     if (bytes <= scratch_bytes) return GRANITE_CUDA_SUCCESS;
     if (capturing()) return refuse_growth("scratch arena");
-    size_t want = bytes + bytes / 4;
-    void* grown = nullptr;
-    if (cudaMalloc(&grown, want) != cudaSuccess) {
-        cudaGetLastError();
-        return fail(GRANITE_CUDA_OUT_OF_MEMORY, "scratch arena: cudaMalloc failed");
-    }
-    void* old = scratch;
-    scratch = grown;
-    scratch_bytes = want;
-    return retire(old);
+    return grow(&scratch, &scratch_bytes, bytes + bytes / 4, 1, "scratch arena");
 }
 
 int granite_cuda_compute::ensure_page_counters(size_t count) {
     if (count <= pages_done_count) return GRANITE_CUDA_SUCCESS;
     if (capturing()) return refuse_growth("decode page counters");
-    const size_t want = count + count / 4 + 1024;
-    int* grown = nullptr;
-    if (cudaMalloc(&grown, want * sizeof(int)) != cudaSuccess) {
+    void* held = d_pages_done;
+    const int rc = grow(&held, &pages_done_count, count + count / 4 + 1024, sizeof(int), "decode page counters");
+    d_pages_done = static_cast<int*>(held);
+    if (rc) return rc;
+    if (cudaMemsetAsync(d_pages_done, 0, pages_done_count * sizeof(int), stream) != cudaSuccess) {
         cudaGetLastError();
-        return fail(GRANITE_CUDA_OUT_OF_MEMORY, "decode page counters: cudaMalloc failed");
-    }
-    if (cudaMemsetAsync(grown, 0, want * sizeof(int), stream) != cudaSuccess) {
-        cudaGetLastError();
-        cudaFree(grown);
+        pages_done_count = 0;  // not to be counted in
         return fail(GRANITE_CUDA_EXECUTION_FAILED, "decode page counters: clearing failed");
     }
-    void* old = d_pages_done;
-    d_pages_done = grown;
-    pages_done_count = want;
-    return retire(old);
+    return GRANITE_CUDA_SUCCESS;
 }
 
 const CUtensorMap* granite_cuda_compute::encode_map(const TensorMapKey& key) {

@@ -81,7 +81,7 @@ struct granite_cuda_compute {
     bool captured = false;  // a call has been made while the stream was capturing
     bool capturing();       // whether it is now (and notes that it was)
     std::vector<void*> retired;
-    int retire(void* old);
+    int grow(void** held, size_t* count, size_t want, size_t unit, const char* what);
     // Cached TMA descriptors, keyed by (buffer, shape).  Bounded: once kMaxTensorMaps entries exist,
     // everything but the kKeepRecent most recently used ones is dropped (encode_map), so a pointer
     // returned by encode_map stays valid for at least the next kKeepRecent - 1 calls to it.

@@ -72,3 +72,45 @@ def test_workspaces_do_not_grow_inside_a_capture(mode, warm):
     del graph, graph2
     o.shutdown()
     fresh.shutdown()
+
+
+@pytest.mark.gpu
+def test_scratch_grows_in_place_near_the_end_of_the_memory():
+    """Growing needs room for the new arena, not for both.  What room is left is what the first arena and the calls need, less than the
+    second arena takes by itself."""
+    import torch
+    import granite_b200 as g
+    torch.cuda.empty_cache()
+    hq, hkv, d = 32, 8, 128
+    o = g.CudaCompute(0)
+    kv = torch.randn((hkv, 256, d), device=DEV).half()
+    rows = (16384, 24576, 65536)  # 335, 503 and 1342 MB of scratch: fp16 hi + lo, and a quarter more
+    q = torch.randn((rows[2], hq, d), device=DEV)
+    out = torch.zeros_like(q)
+
+    def call(n):  # prompt rows far behind a short cache: every row sees all 256 keys
+        o.multihead_attention(q, kv, kv, out, hq, hkv, n, 256, d, d ** -0.5, 256, start_pos=256)
+        o.sync()
+
+    torch.cuda.synchronize()
+    call(rows[0])
+    want = out[:rows[0]].cpu()
+    room = 400 << 20
+    hog = torch.empty(torch.cuda.mem_get_info(0)[0] - room, dtype=torch.uint8, device=DEV)
+    try:
+        assert torch.cuda.mem_get_info(0)[0] < rows[1] * hq * d * 5
+        out.zero_()
+        torch.cuda.synchronize()
+        call(rows[1])
+        assert torch.allclose(out[:rows[0]].cpu(), want, rtol=1e-4, atol=1e-6)
+        # no room at all: refused, and the object works once there is
+        with pytest.raises(g.GraniteCudaError) as e:
+            call(rows[2])
+        assert e.value.code == g.ErrorCode.OutOfMemory
+        call(rows[0])
+    finally:
+        del hog
+        torch.cuda.empty_cache()
+    call(rows[2])
+    assert torch.allclose(out[:rows[0]].cpu(), want, rtol=1e-4, atol=1e-6) and bool(torch.isfinite(out).all())
+    o.shutdown()
