@@ -64,7 +64,7 @@
 namespace gb200 {
 
 constexpr int kTcThreads = 384;
-constexpr int kT = 128;                      // query rows per tile, keys per K/V tile, head_dim
+constexpr int kT = kTileRows;                // 128: query rows per tile, keys per K/V tile, head_dim
 constexpr int kTileBytes = kT * kT * 2;      // 32 KB: one [128 x 128] fp16 tile
 constexpr int kChunkBytes = kTileBytes / 2;  // 16 KB: one 64-column (128-byte) swizzle block
 constexpr int kNodeSlots = 64;               // tree nodes per sequence the kernel is laid out for
@@ -122,27 +122,9 @@ struct TcWindowItem : TcItem {
     int j0;      // first of the item's steps in the query block's
     int chunk;
 };
-// The steps of the query block that starts at row q0: tiles of the sinks, then from the window of its first row to its diagonal.
-struct WindowSteps {
-    int n, n_sink, w0, lo;
-};
-__host__ __device__ __forceinline__ WindowSteps window_steps(const TcParams& p, int q0) {
-    WindowSteps w;
-    const int rows = p.seq_q - q0 < kT ? p.seq_q - q0 : kT, last = p.start_pos + q0 + rows;
-    const int tiles = ((p.seq_kv < last ? p.seq_kv : last) + kT - 1) / kT;  // up to the last visible key
-    w.lo = window_span(p.start_pos + q0, p.window, p.sinks).lo;
-    w.w0 = w.lo / kT < tiles ? w.lo / kT : tiles;
-    const int sink_tiles = ((p.sinks < w.lo ? p.sinks : w.lo) + kT - 1) / kT;
-    w.n_sink = sink_tiles < w.w0 ? sink_tiles : w.w0;
-    w.n = w.n_sink + tiles - w.w0;
-    if (w.n < 1) {  // a block that sees nothing still runs one, masked, step
-        w.n = 1;
-        w.w0 = 0;
-    }
-    return w;
+GB_HOST_DEVICE WindowSteps window_steps(const TcParams& p, int q0) {
+    return window_steps(PrefillSpan{p.seq_q, p.seq_kv, p.start_pos, p.window, p.sinks}, q0);
 }
-// Steps [chunk_begin(n, c), chunk_begin(n, c + 1)) of n are chunk c's; there are more chunks than steps in short blocks.
-__host__ __device__ __forceinline__ int chunk_begin(int n, int n_chunks, int c) { return n * c / n_chunks; }
 // K/V tile of step j
 __device__ __forceinline__ int tile_of(const TcItem&, int j) { return j; }
 __device__ __forceinline__ int tile_of(const TcWindowItem& it, int j) {

@@ -6,6 +6,8 @@
 #include <cuda_fp8.h>
 #include <stdint.h>
 
+#include "view_plan.h"
+
 namespace gb200 {
 
 enum : int { kElemF16 = 0, kElemInt8 = 1, kElemE4M3 = 2 };  // what a cache holds; 1 + cache_dtype for the 8-bit ones
@@ -38,18 +40,6 @@ __device__ __forceinline__ uint32_t q8_encode4(float4 x) {
     }
     return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x.x, x.y), __NV_SATFINITE, __NV_E4M3) |
            ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x.z, x.w), __NV_SATFINITE, __NV_E4M3) << 16);
-}
-
-// What a sliding window leaves of a sequence whose query sits at position `pos`: keys [0, sinks_end) and
-// [lo, pos], sinks_end <= lo.  window 0: no window (sinks_end = lo = 0).
-struct WindowSpan {
-    int sinks_end, lo;
-};
-__host__ __device__ __forceinline__ WindowSpan window_span(int pos, int window, int sinks) {
-    WindowSpan s;
-    s.lo = window > 0 && pos >= window ? pos - window + 1 : 0;
-    s.sinks_end = sinks < s.lo ? sinks : s.lo;
-    return s;
 }
 
 }  // namespace gb200

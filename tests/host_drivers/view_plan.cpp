@@ -1,0 +1,23 @@
+// Test drivers of csrc/view_plan.h, which the kernels and their launchers share; built with the host compiler alone.
+#include "../../granite_b200/csrc/view_plan.h"
+
+using namespace gb200;
+
+extern "C" {
+
+void view_window_span(int pos, int window, int sinks, int* out) {
+    const WindowSpan s = window_span(pos, window, sinks);
+    out[0] = s.sinks_end;
+    out[1] = s.lo;
+}
+
+void view_window_steps(int seq_q, int seq_kv, int start_pos, int window, int sinks, int q0, int* out) {
+    const WindowSteps w = window_steps(PrefillSpan{seq_q, seq_kv, start_pos, window, sinks}, q0);
+    out[0] = w.n;
+    out[1] = w.n_sink;
+    out[2] = w.w0;
+    out[3] = w.lo;
+}
+
+int view_chunk_begin(int n, int n_chunks, int c) { return chunk_begin(n, n_chunks, c); }
+}

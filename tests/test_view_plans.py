@@ -1,0 +1,70 @@
+"""The index arithmetic behind the windowed and 8-bit calls (csrc/view_plan.h, the header that the kernels are compiled from), run on
+the host against the definitions.  Built with the sanitizer for undefined arithmetic: an overflow ends the test."""
+import ctypes as C
+import shutil
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+import view_reference as R
+
+SOURCE = Path(__file__).resolve().parent / "host_drivers" / "view_plan.cpp"
+
+
+@pytest.fixture(scope="module")
+def plans(tmp_path_factory):
+    cxx = shutil.which("g++")
+    if cxx is None:
+        pytest.skip("no C++ compiler")
+    lib = tmp_path_factory.mktemp("view_plan") / "view_plan.so"
+    subprocess.run([cxx, "-std=c++17", "-O1", "-Wall", "-fsanitize=signed-integer-overflow", "-fsanitize-undefined-trap-on-error", "-shared", "-fPIC",
+                    "-o", str(lib), str(SOURCE)], check=True)
+    return C.CDLL(str(lib))
+
+
+def _ints(fn, n, *args):
+    out = (C.c_int * n)()
+    fn(*args, out)
+    return list(out)
+
+
+def test_window_span_is_the_definition(plans):
+    for window in (0, 1, 2, 5, 16, 100, 0x7fffffff):
+        for sinks in (0, 1, 7, 40, 0x7fffffff):
+            for pos in range(0, 60):
+                end, lo = _ints(plans.view_window_span, 2, pos, window, sinks)
+                assert 0 <= end <= lo or lo == end == 0
+                keys = sorted(set(range(end)) | set(range(lo, pos + 1)))
+                assert np.array_equal(np.nonzero(R.visible([pos], pos + 1, window, sinks)[0])[0], keys)
+    assert _ints(plans.view_window_span, 2, 2 ** 31 - 65537, 7, 0x7fffffff) == [2 ** 31 - 65543] * 2
+
+
+def test_window_steps_walk_every_visible_tile_once(plans):
+    rng = np.random.default_rng(1)
+    for i in range(400):
+        seq_q, start = int(rng.integers(1, 700)), int(rng.choice([0, rng.integers(0, 2000)]))
+        end = start + seq_q
+        seq_kv = end if i % 3 else max(1, end - int(rng.integers(0, 900)))
+        window = int(rng.choice([0, 1, 17, 128, rng.integers(1, 1500), 0x7fffffff]))
+        sinks = int(rng.choice([0, 3, 128, 200, rng.integers(0, 900), 0x7fffffff])) if window else 0
+        for q0 in range(0, seq_q, 128):
+            pos = start + np.arange(q0, min(q0 + 128, seq_q))
+            seen = R.visible(pos, seq_kv, window, sinks).any(0)
+            n, n_sink, w0, lo = _ints(plans.view_window_steps, 4, seq_q, seq_kv, start, window, sinks, q0)
+            tiles = [j if j < n_sink else j - n_sink + w0 for j in range(n)]
+            assert n >= 1 and tiles == sorted(set(tiles))
+            need = sorted(set(np.nonzero(seen)[0] // 128))
+            # every tile with a visible key, and no other: but for the tile that a cache ends in before the window begins, and for the one
+            # step of a block that sees nothing
+            assert set(need) <= set(tiles) and set(tiles) - set(need) <= ({seq_kv // 128} if need and lo >= seq_kv else set() if need else {0, seq_kv // 128})
+            hidden = np.nonzero(~seen[: min(lo, seq_kv)])[0]
+            assert np.array_equal(hidden, np.arange(min(sinks, lo, seq_kv), min(lo, seq_kv)))  # what the kernel clears
+
+
+def test_chunks_share_out_every_step(plans):
+    for n in (1, 2, 5, 31, 32, 33, 1000, 1 << 24):
+        for chunks in (1, 2, 3, 24, 32):
+            at = [plans.view_chunk_begin(n, chunks, c) for c in range(chunks + 1)]
+            assert at[0] == 0 and at[-1] == n and all(0 <= b - a <= -(-n // chunks) for a, b in zip(at, at[1:]))
