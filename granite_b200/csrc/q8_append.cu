@@ -114,15 +114,13 @@ __global__ void __launch_bounds__(kAppendThreads) q8_append_kernel(const __grid_
     const long long b = task / p.pages_per_seq;
     const int start = p.positions ? p.positions[b] : p.start_pos;
     const long long room = min((long long)p.table_len, (long long)p.max_blocks * p.block_size);
-    const int lo = max(start, 0);
-    const int hi = (int)min((long long)start + p.new_len, room);
     if (pi == 0 && h == 0 && !is_v && tid == 0 && (start < 0 || (long long)start + p.new_len > room))
         atomicOr(p.status, kStatusBadSeqLen);
-    const int logical = lo / p.block_size + pi;
-    const long long page0 = (long long)logical * p.block_size;  // position of the page's row 0
-    const int r0 = (int)max(lo - page0, 0LL), r1 = (int)min(hi - page0, (long long)p.block_size);
+    const AppendRows rows = append_rows(start, p.new_len, room, p.block_size, pi);
+    const int r0 = rows.r0, r1 = rows.r1;
     if (r0 >= r1) return;
-    const int phys = p.tables[(size_t)b * p.max_blocks + logical];
+    const long long page0 = rows.page * p.block_size;  // position of the page's row 0
+    const int phys = p.tables[(size_t)b * p.max_blocks + rows.page];
     if (phys < 0 || phys >= p.num_blocks) {
         if (tid == 0) atomicOr(p.status, kStatusBadTable);
         return;

@@ -52,4 +52,22 @@ GB_HOST_DEVICE WindowSteps window_steps(const PrefillSpan& p, int q0) {
 // Steps [chunk_begin(n, c), chunk_begin(n, c + 1)) of n are chunk c's; there are more chunks than steps in short blocks.
 GB_HOST_DEVICE int chunk_begin(int n, int n_chunks, int c) { return n * c / n_chunks; }
 
+// The rows [r0, r1) of logical page `page` that an append of new_len tokens from position `start` writes, page the touched-th from the first
+// page with a place for one of them: none (r0 >= r1) where `start` leaves no token in [0, room).  Any start may come, so everything is in
+// 64 bits and brought into the page before it is narrowed.
+struct AppendRows {
+    long long page;
+    int r0, r1;
+};
+GB_HOST_DEVICE AppendRows append_rows(long long start, long long new_len, long long room, int block_size, int touched) {
+    const long long lo = start > 0 ? start : 0, hi = start + new_len < room ? start + new_len : room;
+    AppendRows a;
+    a.page = lo / block_size + touched;
+    const long long page0 = a.page * block_size;
+    const long long r0 = lo - page0, r1 = hi - page0;
+    a.r0 = (int)(r0 < 0 ? 0 : r0 < block_size ? r0 : block_size);
+    a.r1 = (int)(r1 < 0 ? 0 : r1 < block_size ? r1 : block_size);
+    return a;
+}
+
 }  // namespace gb200

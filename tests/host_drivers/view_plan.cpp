@@ -19,5 +19,12 @@ void view_window_steps(int seq_q, int seq_kv, int start_pos, int window, int sin
     out[3] = w.lo;
 }
 
+void view_append_rows(long long start, long long new_len, long long room, int block_size, int touched, long long* out) {
+    const AppendRows a = append_rows(start, new_len, room, block_size, touched);
+    out[0] = a.page;
+    out[1] = a.r0;
+    out[2] = a.r1;
+}
+
 int view_chunk_begin(int n, int n_chunks, int c) { return chunk_begin(n, n_chunks, c); }
 }

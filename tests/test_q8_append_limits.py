@@ -1,0 +1,35 @@
+"""The 8-bit append at the limits of its arguments: positions at the ends of the 32-bit range, sizes that no index may pass."""
+import numpy as np
+import pytest
+
+import view_reference as R
+from test_q8_cache import _append_reference, _check_append, _rotate32, _rope_tables, _run_append
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", [0, 1])
+@pytest.mark.parametrize("block_size,d", [(16, 128), (16, 64), (1, 40), (5, 8)])
+def test_append_with_positions_at_the_ends_of_the_range(compute, cache_dtype, block_size, d):
+    """Positions that no table can hold are skipped and reported, the sequences beside them are written as ever."""
+    from granite_b200.capi import ErrorCode
+    rng = np.random.default_rng(block_size)
+    positions = np.array([2 ** 31 - 1, 3, 2 ** 31 - 200, -(2 ** 31), 0, 2 ** 30, -1], np.int32)
+    hkv, n, limit = 2, 300, 320
+    pages = -(-limit // block_size)
+    tables = np.arange(len(positions) * pages, dtype=np.int32).reshape(len(positions), pages)
+    blocks = tables.size
+    pools = [R.random_pool(rng, blocks, block_size, hkv, d, cache_dtype) for _ in range(2)]
+    codes, scales = [p[0] for p in pools], [p[1] for p in pools]
+    k, v = (rng.standard_normal((len(positions), n, hkv, d), dtype=np.float32) for _ in range(2))
+    q = rng.standard_normal((len(positions), n, 2, d), dtype=np.float32)
+    cos, sin = _rope_tables(limit, d)
+    got = _run_append(compute, q, k, v, cos, sin, codes, scales, tables, positions, block_size, cache_dtype)
+    assert got[3] is not None and got[3].code == ErrorCode.InvalidArgument
+    where = positions[:, None].astype(np.int64) + np.arange(n)
+    ok, at = ((where >= 0) & (where < limit))[:, :, None, None], np.clip(where, 0, limit - 1)
+    want_codes, want_scales = [c.copy() for c in codes], [s.copy() for s in scales]
+    for x, c, s in ((_rotate32(k, cos[at][:, :, None], sin[at][:, :, None]), want_codes[0], want_scales[0]), (v, want_codes[1], want_scales[1])):
+        _append_reference(x, c, s, tables, positions, block_size, cache_dtype, limit)
+    _check_append(got, (want_codes, want_scales))
+    assert np.array_equal(got[0], np.where(ok, _rotate32(q, cos[at][:, :, None], sin[at][:, :, None]), q))
+    compute.sync()

@@ -68,3 +68,26 @@ def test_chunks_share_out_every_step(plans):
         for chunks in (1, 2, 3, 24, 32):
             at = [plans.view_chunk_begin(n, chunks, c) for c in range(chunks + 1)]
             assert at[0] == 0 and at[-1] == n and all(0 <= b - a <= -(-n // chunks) for a, b in zip(at, at[1:]))
+
+
+def test_append_rows_cover_what_can_be_placed_and_nothing_else(plans):
+    """Every start a 32-bit position can name, the ends of the range among them: the pages that a call touches (as many as the launch has
+    blocks for) hold exactly the positions of [start, start + new_len) that lie in [0, room)."""
+    fn = plans.view_append_rows
+    rng = np.random.default_rng(2)
+    far = [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 200, 2 ** 30, -1, -7, -300, -(2 ** 31)]
+    for bs in (1, 5, 16, 48, 1 << 20):
+        for new_len in (1, 2, 16, 17, 300):
+            for start in far + [0, 1, 15, 16, 47, 63, 64] + [int(x) for x in rng.integers(0, 400, 5)]:
+                room = int(rng.integers(1, 400))
+                pages = (new_len + bs - 2) // bs + 1
+                got = []
+                for i in range(pages):
+                    out = (C.c_longlong * 3)()
+                    fn(C.c_longlong(start), C.c_longlong(new_len), C.c_longlong(room), bs, i, out)
+                    page, r0, r1 = out
+                    assert 0 <= r0 <= bs and 0 <= r1 <= bs
+                    if r0 < r1:
+                        assert 0 <= page <= (room - 1) // bs
+                        got += range(page * bs + r0, page * bs + r1)
+                assert got == list(range(max(start, 0), max(min(start + new_len, room), max(start, 0))))
