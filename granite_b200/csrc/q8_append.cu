@@ -243,6 +243,9 @@ int check_q8_append(const GraniteCudaRopeAppendArgs& a, const GraniteCudaQ8Cache
     if (a.batch_size >= limit || a.new_len >= limit || a.num_heads > 65535 || a.num_kv_heads > 65535 || a.block_size >= limit ||
         a.max_blocks_per_seq >= limit || a.num_blocks >= limit || a.table_len >= limit || a.start_pos >= limit)
         return fail(GRANITE_CUDA_INVALID_ARGUMENT, "rope_paged_kv_cache_append_q8: a size is out of range (65535 heads, 2^31 - 1 otherwise)");
+    // the kernel counts the four-element pieces of a page's head in 32 bits, a block's stride beyond the last
+    if ((uint64_t)a.block_size * (a.head_dim / 4) >= limit - 65536)
+        return fail(GRANITE_CUDA_INVALID_ARGUMENT, "rope_paged_kv_cache_append_q8: block_size * head_dim is out of range (below about 2^33)");
     return GRANITE_CUDA_SUCCESS;
 }
 

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import view_reference as R
-from test_q8_cache import _append_reference, _check_append, _rotate32, _rope_tables, _run_append
+from test_q8_cache import _append_args, _append_reference, _check_append, _refusal, _rotate32, _rope_tables, _run_append
 
 
 @pytest.mark.gpu
@@ -33,3 +33,14 @@ def test_append_with_positions_at_the_ends_of_the_range(compute, cache_dtype, bl
     _check_append(got, (want_codes, want_scales))
     assert np.array_equal(got[0], np.where(ok, _rotate32(q, cos[at][:, :, None], sin[at][:, :, None]), q))
     compute.sync()
+
+
+@pytest.mark.parametrize("block_size,head_dim", [(1 << 25, 256), ((1 << 31) - 1, 8), (1 << 26, 128), ((1 << 30) - 32768, 8)])
+def test_a_page_whose_pieces_pass_32_bits_is_refused(block_size, head_dim):
+    """Rows of a page times its four-element pieces are counted in 32 bits; the last case is the first size that is refused."""
+    from granite_b200 import capi
+    args = _append_args(block_size=block_size, head_dim=head_dim, max_blocks_per_seq=1, num_blocks=1)
+    got, text = _refusal(capi.lib.granite_cuda_rope_paged_kv_cache_append_q8, *args)
+    assert got.name == "InvalidArgument" and "block_size" in text
+    got, text = _refusal(capi.lib.granite_cuda_rope_paged_kv_cache_append_q8, *_append_args(block_size=(1 << 30) - 32769, head_dim=8))
+    assert got.name == "NullPointer" and "compute object" in text  # nothing left to refuse but the missing object
