@@ -1022,7 +1022,6 @@ static int launch_tc(granite_cuda_compute* c, TcKernel kern, const char* name, i
 }
 
 // out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the chunks of a row, in chunk order; one warp per (row, head).
-constexpr int kMaxChunks = 32;  // one per lane
 __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constant__ TcParams p, int hd) {
     const int lane = threadIdx.x & 31;
     const size_t idx = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);  // (sequence, row, head)
@@ -1067,35 +1066,35 @@ __global__ void __launch_bounds__(256) prefill_merge_kernel(const __grid_constan
         *reinterpret_cast<float4*>(static_cast<float*>(p.out) + idx * hd + lane * 4) = acc;
 }
 
-// How many chunks an item's tiles are cut into.  The estimate is the longest queue of any SM - items come in rounds of one per
-// SM, a chunk costs its steps and about one and a half more to start and drain - plus the merge's launch and traffic, at
-// 1.35 us a step.  An fp32 output additionally wants no more than 22 tiles in one accumulator (see the top of the file).
-// Returns the bytes of partials; fills n_chunks.
-static size_t plan_chunks(granite_cuda_compute* c, TcParams& p, int hd) {
-    const long long items = (long long)p.n_qblocks * p.batch * p.num_kv_heads * p.units_per_kvh;
-    int longest = 1;
-    for (int b = 0; b < p.n_qblocks; b += 1 + p.n_qblocks / 64) longest = std::max(longest, window_steps(p, b * kT).n);
-    longest = std::max(longest, window_steps(p, (p.n_qblocks - 1) * kT).n);
-    const double rows = (double)p.batch * p.seq_q * p.num_heads;
-    double best = 0;
-    p.n_chunks = 1;
-    static const int choices[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, kMaxChunks};
-    bool chosen = false;
-    for (int n : choices) {
-        if (n > longest || items * n >= (1ll << 31)) break;
-        if (n > 1 && rows * n * (hd * 4 + 8) > 16e9) break;  // partials of more than 16 GB: the accuracy of a long run instead
-        const int steps = (longest + n - 1) / n;
-        if (!p.out_fp16 && steps > 22 && n < kMaxChunks && n < longest) continue;
-        const double rounds = (double)((items * n + c->sm_count - 1) / c->sm_count);
-        const double us = rounds * (steps + 1.5) * 1.35 + (n > 1 ? 3.0 + rows * n * hd * 8 / 5e6 : 0.0);
-        if (!chosen || us < best) {
-            best = us;
-            p.n_chunks = n;
-            chosen = true;
-        }
+static ChunkProblem chunk_problem(granite_cuda_compute* c, const TcParams& p) {
+    return ChunkProblem{{p.seq_q, p.seq_kv, p.start_pos, p.window, p.sinks}, p.batch, p.num_heads, p.d_chunks * 64, c->sm_count, p.out_fp16 != 0};
+}
+static size_t partial_bytes(const TcParams& p) {
+    return p.n_chunks == 1 ? 0 : (size_t)p.batch * p.seq_q * p.num_heads * p.n_chunks * (p.d_chunks * 64 * sizeof(float) + sizeof(float2)) + 256;
+}
+// Scratch for `fixed` bytes and the partials; where there is no room for these, the call runs in one chunk (see kMaxTilesF32 for what that
+// costs a long one).
+static int ensure_with_partials(granite_cuda_compute* c, TcParams& p, size_t fixed) {
+    int rc = c->ensure_scratch(fixed + partial_bytes(p));
+    if (rc == GRANITE_CUDA_OUT_OF_MEMORY && p.n_chunks > 1) {
+        p.n_chunks = 1;
+        rc = c->ensure_scratch(fixed);
     }
-    if (p.n_chunks == 1) return 0;
-    return (size_t)rows * p.n_chunks * (hd * 4 + sizeof(float2)) + 256;
+    return rc;
+}
+// A call whose partials pass the limit runs as several, each on some of the query rows.
+template <typename Args, typename Launch>
+static int launch_by_rows(const Args& a, uint32_t rows, Launch launch) {
+    const size_t elements = (size_t)a.num_heads * a.head_dim;
+    for (uint32_t s0 = 0; s0 < a.seq_q; s0 += rows) {
+        Args part = a;
+        part.q = static_cast<const char*>(a.q) + s0 * elements * (a.q_dtype == 0 ? 4 : 2);
+        part.output = static_cast<char*>(a.output) + s0 * elements * (a.out_dtype == 0 ? 4 : 2);
+        part.start_pos = a.start_pos + s0;
+        part.seq_q = std::min(rows, a.seq_q - s0);
+        if (int rc = launch(part)) return rc;
+    }
+    return GRANITE_CUDA_SUCCESS;
 }
 static void place_partials(TcParams& p, uint8_t* at, int hd) {
     if (p.n_chunks == 1) return;
@@ -1117,11 +1116,11 @@ static void set_window(TcParams& p, const CacheView& view) {
     p.sinks = (int)std::min(view.sinks, 0x7fffffffu);
 }
 
-// fp32 queries -> hi / lo fp16 arrays at the start of the scratch arena, which is made large enough for `behind` bytes after them
+// fp32 queries -> hi / lo fp16 arrays at the start of the scratch arena
 static size_t split_bytes(size_t n) { return 2 * ((n * 2 + 255) / 256 * 256); }
-static int split_queries(granite_cuda_compute* c, const void* q, size_t n, const void** hi_out, const void** lo_out, size_t behind = 0) {
+static int split_queries(granite_cuda_compute* c, const void* q, size_t n, const void** hi_out, const void** lo_out) {
     const size_t half_bytes = split_bytes(n) / 2;
-    int rc = c->ensure_scratch(2 * half_bytes + behind);
+    int rc = c->ensure_scratch(2 * half_bytes);
     if (rc) return rc;
     LaunchScope t(c, "split_q_f16");
     __half* hi = static_cast<__half*>(c->scratch);
@@ -1169,18 +1168,36 @@ int launch_prefill(granite_cuda_compute* c, const GraniteCudaAttentionArgs& a, c
     p.start_pos = (int)a.start_pos;
 
     p.n_chunks = 1;
-    size_t partials = 0;
     if (view.window > 0) {
         set_window(p, view);
-        partials = plan_chunks(c, p, (int)D);
+        const ChunkProblem cp = chunk_problem(c, p);
+        const uint32_t rows = (uint32_t)rows_per_launch(cp);
+        if (rows < a.seq_q && batch == 1) return launch_by_rows(a, rows, [&](const GraniteCudaAttentionArgs& part) { return launch_prefill(c, part, view); });
+        if (rows < a.seq_q) {  // the rows of a batch are not contiguous: sequence by sequence
+            for (uint32_t b = 0; b < batch; b++) {
+                GraniteCudaAttentionArgs one = a;
+                const size_t row0 = (size_t)b * a.seq_q * a.num_heads * D, kv0 = (size_t)b * a.num_kv_heads * max_seq * D;
+                one.q = static_cast<const char*>(a.q) + row0 * (a.q_dtype == 0 ? 4 : 2);
+                one.output = static_cast<char*>(a.output) + row0 * (a.out_dtype == 0 ? 4 : 2);
+                one.k = static_cast<const char*>(a.k) + kv0 * 2;
+                one.v = static_cast<const char*>(a.v) + kv0 * 2;
+                one.max_seq = max_seq;
+                one.batch_size = 1;
+                if (int rc = launch_prefill(c, one, view)) return rc;
+            }
+            return GRANITE_CUDA_SUCCESS;
+        }
+        p.n_chunks = plan_chunks(cp);
     }
     const bool split_q = a.q_dtype == 0;
     const void *q16 = a.q, *q16_lo = a.q;
     const size_t n_q = (size_t)batch * a.seq_q * a.num_heads * D;
-    if (split_q || partials) {
-        int rc = split_q ? split_queries(c, a.q, n_q, &q16, &q16_lo, partials) : c->ensure_scratch(partials);
+    if (split_q || p.n_chunks > 1) {
+        const size_t q_bytes = split_q ? split_bytes(n_q) : 0;
+        int rc = ensure_with_partials(c, p, q_bytes);
+        if (rc == GRANITE_CUDA_SUCCESS && split_q) rc = split_queries(c, a.q, n_q, &q16, &q16_lo);
         if (rc) return rc;
-        place_partials(p, static_cast<uint8_t*>(c->scratch) + (split_q ? split_bytes(n_q) : 0), (int)D);
+        place_partials(p, static_cast<uint8_t*>(c->scratch) + q_bytes, (int)D);
     }
 
     const uint64_t q_rows = (uint64_t)batch * a.seq_q;
@@ -1237,18 +1254,22 @@ int launch_paged_prefill(granite_cuda_compute* c, const GraniteCudaPagedPrefillA
     p.num_blocks = (int)a.num_blocks;
 
     p.n_chunks = 1;
-    size_t partials = 0;
     if (view.window > 0) {
         set_window(p, view);
-        partials = plan_chunks(c, p, (int)D);
+        const ChunkProblem cp = chunk_problem(c, p);
+        const uint32_t rows = (uint32_t)rows_per_launch(cp);
+        if (rows < a.seq_q) return launch_by_rows(a, rows, [&](const GraniteCudaPagedPrefillArgs& part) { return launch_paged_prefill(c, part, view); });
+        p.n_chunks = plan_chunks(cp);
     }
     const bool split_q = a.q_dtype == 0;
     const void *q16 = a.q, *q16_lo = a.q;
     const size_t n_q = (size_t)a.seq_q * a.num_heads * D;
-    if (split_q || partials) {
-        int rc = split_q ? split_queries(c, a.q, n_q, &q16, &q16_lo, partials) : c->ensure_scratch(partials);
+    if (split_q || p.n_chunks > 1) {
+        const size_t q_bytes = split_q ? split_bytes(n_q) : 0;
+        int rc = ensure_with_partials(c, p, q_bytes);
+        if (rc == GRANITE_CUDA_SUCCESS && split_q) rc = split_queries(c, a.q, n_q, &q16, &q16_lo);
         if (rc) return rc;
-        place_partials(p, static_cast<uint8_t*>(c->scratch) + (split_q ? split_bytes(n_q) : 0), (int)D);
+        place_partials(p, static_cast<uint8_t*>(c->scratch) + q_bytes, (int)D);
     }
 
     const CUtensorMap* qmap = c->tensor_map_2d(q16, (uint64_t)a.num_heads * D, a.seq_q, (uint64_t)a.num_heads * D * 2, 64, kT, 128);
@@ -1421,11 +1442,13 @@ int launch_paged_prefill_q8(granite_cuda_compute* c, const GraniteCudaPagedPrefi
     const size_t q_bytes = split_q ? split_bytes(n_q) + step_bytes : 0;
     const size_t kv_bytes = (size_t)g.hkv * g.rows * D * 2;                                           // a multiple of 128 rows * 128 bytes
     const size_t page_bytes = ((size_t)g.hkv * g.page_stride * 4 + 255) / 256 * 256;
-    const size_t partials = plan_chunks(c, p, (int)D);
+    const ChunkProblem cp = chunk_problem(c, p);
+    const uint32_t rows = (uint32_t)rows_per_launch(cp);
+    if (rows < a.seq_q) return launch_by_rows(a, rows, [&](const GraniteCudaPagedPrefillArgs& part) { return launch_paged_prefill_q8(c, part, view); });
+    p.n_chunks = plan_chunks(cp);
     const size_t fixed = 2 * kv_bytes + 3 * page_bytes + ((size_t)g.hkv * 4 + 255) / 256 * 256;
-    const size_t behind = fixed + partials;
     const void *q16 = a.q, *q16_lo = a.q;
-    int rc = c->ensure_scratch(q_bytes + behind);
+    int rc = ensure_with_partials(c, p, q_bytes + fixed);
     if (rc) return rc;
     if (split_q) {
         uint8_t* at = static_cast<uint8_t*>(c->scratch);

@@ -500,7 +500,9 @@ int granite_cuda_batched_paged_attention_decode_q8(granite_cuda_compute_t* c, co
                                                    const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window);
 
 /* granite_cuda_paged_prefill_attention over the 8-bit cache; window may be NULL.  Same shapes as the fp16 call.  The visible
- * codes are laid out as fp16 in the object's scratch first (4 bytes per key, KV head and dim). */
+ * codes are laid out as fp16 in the object's scratch first (4 bytes per key, KV head and dim), and the keys may be cut into
+ * chunks whose partial results, up to 1 GiB of them, are kept there too; a call that would need more runs as several
+ * launches over some of its rows each. */
 int granite_cuda_paged_prefill_attention_q8(granite_cuda_compute_t* c, const GraniteCudaPagedPrefillArgs* args,
                                             const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window);
 
@@ -508,7 +510,8 @@ int granite_cuda_paged_prefill_attention_q8(granite_cuda_compute_t* c, const Gra
  * The three calls without the suffix, restricted to the keys that the window leaves visible.  A sequence's query
  * positions are those of the plain calls (decode: the last token; prefill: start_pos + i).  Pages that no query of the
  * call sees are not read and their table entries are not looked at, so a host may free them.  A query row that sees no
- * key at all (contiguous prefill with seq_kv short of the window's start) gets zeros. */
+ * key at all (contiguous prefill with seq_kv short of the window's start) gets zeros.  Prefill keeps partial results of keys
+ * that are cut into chunks in the object's scratch, up to 1 GiB (see above). */
 int granite_cuda_batched_paged_attention_decode_window(granite_cuda_compute_t* c, const GraniteCudaPagedDecodeArgs* args,
                                                        const GraniteCudaAttentionWindow* window);
 int granite_cuda_multihead_attention_window(granite_cuda_compute_t* c, const GraniteCudaAttentionArgs* args,

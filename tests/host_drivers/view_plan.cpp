@@ -26,5 +26,18 @@ void view_append_rows(long long start, long long new_len, long long room, int bl
     out[2] = a.r1;
 }
 
+// shape: seq_q, seq_kv, start_pos, window, sinks, batch, num_heads, head_dim, sm_count, out_fp16
+// out: wanted chunks and rows per launch of the call; for its last launch of that many rows: longest item, chunks, bytes of partials
+void view_chunk_plan(const int* s, long long* out) {
+    ChunkProblem c{{s[0], s[1], s[2], s[3], s[4]}, s[5], s[6], s[7], s[8], s[9] != 0};
+    out[0] = wanted_chunks(c);
+    out[1] = rows_per_launch(c);
+    c.span.start_pos += c.span.seq_q - (int)out[1];
+    c.span.seq_q = (int)out[1];
+    out[2] = longest_steps(c.span);
+    out[3] = plan_chunks(c);
+    out[4] = out[3] == 1 ? 0 : (long long)(row_partial_bytes(c) * c.span.seq_q * out[3]);
+}
+
 int view_chunk_begin(int n, int n_chunks, int c) { return chunk_begin(n, n_chunks, c); }
 }

@@ -91,3 +91,43 @@ def test_append_rows_cover_what_can_be_placed_and_nothing_else(plans):
                         assert 0 <= page <= (room - 1) // bs
                         got += range(page * bs + r0, page * bs + r1)
                 assert got == list(range(max(start, 0), max(min(start + new_len, room), max(start, 0))))
+
+
+def _plan(plans, seq_q, start, heads, head_dim=128, out_fp16=False, window=0, sinks=0, batch=1, seq_kv=None, sms=148):
+    shape = (C.c_int * 10)(seq_q, seq_kv or start + seq_q, start, window, sinks, batch, heads, head_dim, sms, int(out_fp16))
+    out = (C.c_longlong * 5)()
+    plans.view_chunk_plan(shape, out)
+    return dict(zip(("wanted", "rows", "longest", "chunks", "bytes"), out))
+
+
+LONG = [(16384, 114688, 64), (32768, 98304, 32), (8192, 57344, 64), (2048, 129024, 32), (2048, 14336, 32), (4001, 4099, 32), (509, 1531, 32), (1, 1000000, 8),
+        (131072, 0, 128), (128, 2000000, 65535), (100, 0, 4)]
+
+
+@pytest.mark.parametrize("seq_q,start,heads", LONG)
+@pytest.mark.parametrize("out_fp16", [False, True])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (4096, 4), (100000, 1000)])
+def test_chunk_plans_bound_the_run_of_an_accumulator_and_the_partials(plans, seq_q, start, heads, out_fp16, window, sinks):
+    """No launch holds more than a GiB of partials; an accumulator takes 22 key tiles for an fp32 output and 128 for an fp16 one, or - over more
+    tiles than 32 chunks of those - a 32nd of the tiles; only where 128 rows of partials pass the limit by themselves are there fewer chunks,
+    and then the most that fit."""
+    p = _plan(plans, seq_q, start, heads, out_fp16=out_fp16, window=window, sinks=sinks)
+    tiles = 128 if out_fp16 else 22
+    assert p["bytes"] <= 1 << 30
+    assert p["rows"] == seq_q or p["rows"] % 128 == 0 and 0 < p["rows"] < seq_q
+    steps = -(-p["longest"] // p["chunks"])
+    row_bytes = heads * (128 * 4 + 8) * 128
+    if row_bytes * p["wanted"] <= 1 << 30:
+        assert steps <= max(tiles, -(-p["longest"] // 32)), (p, steps)
+    else:
+        fits = [n for n in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32) if n == 1 or row_bytes * n <= 1 << 30]
+        assert p["rows"] == min(128, seq_q) and p["chunks"] == max(fits)
+    # rows are only given to several launches when they have to be
+    if p["rows"] < seq_q:
+        assert heads * (128 * 4 + 8) * seq_q * p["wanted"] > 1 << 30
+        assert p["rows"] == 128 or heads * (128 * 4 + 8) * (p["rows"] + 128) * p["wanted"] > 1 << 30
+
+
+def test_chunk_plans_of_short_calls_stay_in_one_launch(plans):
+    for seq_q, start, heads, window in ((2048, 0, 32, 512), (509, 1531, 32, 0), (4001, 4099, 32, 2047), (2048, 14336, 32, 0)):
+        assert _plan(plans, seq_q, start, heads, window=window)["rows"] == seq_q

@@ -114,3 +114,94 @@ def test_scratch_grows_in_place_near_the_end_of_the_memory():
     call(rows[2])
     assert torch.allclose(out[:rows[0]].cpu(), want, rtol=1e-4, atol=1e-6) and bool(torch.isfinite(out).all())
     o.shutdown()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["contiguous", "paged", "q8"])
+def test_a_prefill_of_many_rows_over_a_long_context_runs_in_several_launches(kind):
+    """4096 fp32 rows of 64 heads over 100000 keys want 32 chunks each: more partials than a launch may hold.  The scratch stays bounded, and the
+    rows on both sides of the cuts come out right."""
+    import torch
+    import granite_b200 as g
+    hq, hkv, d, seq, start = 64, 1, 64, 4096, 96000
+    n, scale, window, sinks = seq + start, d ** -0.5, 99000, 8
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(3)
+    q = torch.empty((seq, hq, d), device=DEV).normal_(generator=gen)
+    kv = [torch.empty((1, n, d), device=DEV).normal_(generator=gen).half() for _ in range(2)]
+    out = torch.full_like(q, float("nan"))
+    blocks = (n + 15) // 16
+    table = torch.randperm(blocks, device=DEV, generator=gen).int()
+    o = g.CudaCompute(0)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info(0)[0]
+    if kind == "contiguous":
+        o.multihead_attention_window(q, *kv, out, hq, hkv, seq, n, d, scale, window, sinks, start_pos=start)
+    elif kind == "paged":
+        pools = []
+        for x in kv:
+            p = torch.zeros((blocks, 16, 1, d), device=DEV, dtype=torch.float16)
+            p[table.long()] = torch.nn.functional.pad(x[0], (0, 0, 0, blocks * 16 - n)).view(blocks, 16, 1, d)
+            pools.append(p)
+        torch.cuda.synchronize()
+        free = torch.cuda.mem_get_info(0)[0]
+        o.paged_prefill_attention_window(q, *pools, table, out, hq, hkv, seq, start, d, 16, blocks, blocks, scale, window, sinks)
+    else:
+        codes = [(x[0].float() * 30).round().clamp(-127, 127).to(torch.int8) for x in kv]
+        kv = [(c.double() / 30)[None] for c in codes]
+        pools = []
+        for c in codes:
+            p = torch.zeros((blocks, 16, 1, d), device=DEV, dtype=torch.int8)
+            p[table.long()] = torch.nn.functional.pad(c, (0, 0, 0, blocks * 16 - n)).view(blocks, 16, 1, d)
+            pools.append(p)
+        scales = torch.full((blocks, 1), 1 / 30, device=DEV)
+        torch.cuda.synchronize()
+        free = torch.cuda.mem_get_info(0)[0]
+        o.paged_prefill_attention_q8(q, *pools, scales, scales, table, out, hq, hkv, seq, start, d, 16, blocks, blocks, scale, 0, window=window, sinks=sinks)
+    o.sync()
+    # partials of 1 GiB, the queries' halves, the 8-bit cache's fp16 copy, a quarter more
+    assert free - torch.cuda.mem_get_info(0)[0] <= 1.25 * ((1 << 30) + q.numel() * 4 + 4 * n * d + (1 << 20)) + (64 << 20)
+    k, v = (x[0].double() for x in kv)
+    for rows in (slice(0, 3), slice(1916, 1926), slice(seq - 3, seq)):
+        pos = start + torch.arange(seq, device=DEV)[rows]
+        j = torch.arange(n, device=DEV)
+        seen = (j <= pos[:, None]) & ((pos[:, None] - j < window) | (j < sinks))
+        x = torch.einsum("rhd,nd->rhn", q[rows].double(), k) * scale
+        x.masked_fill_(~seen[:, None], -float("inf"))
+        w = torch.softmax(x, -1)
+        want, mean = w @ v, w @ v.abs()
+        # a 32nd of the tiles in one accumulator, 2.4e-9 for each key, and what any of the calls may be off by (view_reference.assert_close)
+        assert ((out[rows].double() - want).abs() <= mean * (2.4e-9 * n / 32 + 2.0 ** -16.5)).all()
+    o.shutdown()
+
+
+@pytest.mark.gpu
+def test_a_prefill_without_room_for_partials_runs_in_one_chunk():
+    """Few rows over a long context are cut along the keys where the scratch has room, and run in one piece where it has not."""
+    import torch
+    import granite_b200 as g
+    torch.cuda.empty_cache()
+    hq, hkv, d, seq, n = 32, 8, 128, 2048, 16384
+    q = torch.randn((seq, hq, d), device=DEV).half()
+    k, v = (torch.randn((hkv, n, d), device=DEV).half() for _ in range(2))
+    outs = [torch.zeros((seq, hq, d), device=DEV) for _ in range(2)]
+
+    def call(o, out):
+        o.multihead_attention_window(q, k, v, out, hq, hkv, seq, n, d, d ** -0.5, n, 0, q_dtype=1, start_pos=n - seq)
+        o.sync()
+
+    roomy, tight = g.CudaCompute(0), g.CudaCompute(0)
+    torch.cuda.synchronize()
+    before = torch.cuda.mem_get_info(0)[0]
+    call(roomy, outs[0])
+    assert before - torch.cuda.mem_get_info(0)[0] > 150 << 20  # at least six chunks of 34 MB
+    hog = torch.empty(torch.cuda.mem_get_info(0)[0] - (120 << 20), dtype=torch.uint8, device=DEV)
+    try:
+        call(tight, outs[1])
+    finally:
+        del hog
+        torch.cuda.empty_cache()
+    # one run over 128 tiles: 2.4e-9 a key
+    assert float((outs[0] - outs[1]).norm() / outs[0].norm()) <= 2.4e-9 * n
+    roomy.shutdown()
+    tight.shutdown()
