@@ -1314,12 +1314,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                 }
                 if constexpr (kMask) fold(mt, acc);
             }
-            __syncwarp();
+            // Every lane's reads of the slots, and its zeros in rows that are not seen, come before the next copies into them: the fence is
+            // each lane's own and stands before the barrier that lane 0 arrives behind.
+            bool written = kMask;
 #pragma unroll
-            for (int pp = 0; pp < PP; pp++) {
-                if (!has[pp]) continue;
-                if (kMask || ntok[pp] < kPageTokens) fence_proxy_async_smem();
-                if (lane == 0) mbar_arrive(&empty[slot_v[pp]]);
+            for (int pp = 0; pp < PP; pp++) written |= has[pp] && ntok[pp] < kPageTokens;
+            if (written) fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+#pragma unroll
+                for (int pp = 0; pp < PP; pp++)
+                    if (has[pp]) mbar_arrive(&empty[slot_v[pp]]);
             }
         }
 
