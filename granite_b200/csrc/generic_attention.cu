@@ -198,7 +198,9 @@ __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericP
         }
         const float m_chunk = block_max(s, s_red);
         const float m_new = fmaxf(m_run, m_chunk);
-        const float pw = (krow && m_new > -INFINITY) ? __expf(s - m_new) : 0.f;
+        // A view's NaN scores stay NaN, as on the tuned kernels.  (The maximum passes over them: of nothing else it is -infinity.)
+        constexpr bool kView = kElem != kElemF16 || kWindow;
+        const float pw = kView && s != s ? s : (krow && m_new > -INFINITY) ? __expf(s - m_new) : 0.f;
         s_p[tid] = kElem == kElemF16 ? pw : pw * v_scale;
         s_vrow[tid] = vrow;
         const float l_chunk = block_sum(pw, s_red);  // its barriers also publish s_p / s_vrow
@@ -224,7 +226,8 @@ __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericP
     for (int u = 0; u < kGenMaxDim / kGenThreads; u++) {
         const int dim = tid + u * kGenThreads;
         if (dim >= p.d) continue;
-        const float o = l_run > 0.f ? acc[u] / l_run : 0.f;  // an empty sequence gives zeros
+        float o = l_run > 0.f ? acc[u] / l_run : 0.f;  // an empty sequence gives zeros
+        if ((kElem != kElemF16 || kWindow) && l_run != l_run) o = l_run;
         if (p.out_f16) static_cast<__half*>(p.out)[qo + dim] = __float2half_rn(o);
         else static_cast<float*>(p.out)[qo + dim] = o;
     }
