@@ -62,11 +62,14 @@ __device__ __forceinline__ float4 finite_part(float4 x) {
 }
 // x / scale, correctly rounded, from the correctly rounded reciprocal: the quotient estimate and one correction by its exact
 // remainder (Markstein, IBM Journal of Research and Development 34, 1990).  A division per element was two thirds of
-// the kernel's instructions.
+// the kernel's instructions.  The remainder is exact while its last bit is a number: that of q times that of scale, 2^-56 scale for the
+// smallest q that rounds to a code (2^-10).  Below kTinyScale both are multiplied by a power of two first, which changes nothing else.
+constexpr float kTinyScale = 0x1p-90f, kTinyFactor = 0x1p64f;
 __device__ __forceinline__ float over(float x, float scale, float inv) {
     const float q = __fmul_rn(x, inv);
     return fmaf(fmaf(-q, scale, x), inv, q);
 }
+__device__ __forceinline__ float4 times(float4 x, float f) { return make_float4(x.x * f, x.y * f, x.z * f, x.w * f); }
 __device__ __forceinline__ float4 over(float4 x, float scale, float inv) {
     return make_float4(over(x.x, scale, inv), over(x.y, scale, inv), over(x.z, scale, inv), over(x.w, scale, inv));
 }
@@ -202,7 +205,8 @@ __global__ void __launch_bounds__(kAppendThreads) q8_append_kernel(const __grid_
     float need = __fdiv_rn(amax, q8_max<kElem>());
     if (need < 1.17549435e-38f) need = 0.f;  // below the normal range: stored as zeros
     const float scale = fmaxf(before, need);
-    const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;  // (scale 0: every row is zero)
+    const float up = scale < kTinyScale ? kTinyFactor : 1.f, by = scale * up;
+    const float inv = scale > 0.f ? __frcp_rn(by) : 0.f;  // (scale 0: every row is zero)
 
     if (scale > before && r0 > 0) {
         const float ratio = __fdiv_rn(before, scale);
@@ -212,13 +216,17 @@ __global__ void __launch_bounds__(kAppendThreads) q8_append_kernel(const __grid_
         }
     }
     if (kQuads) {
+        if (up != 1.f) {
+#pragma unroll
+            for (int it = 0; it < kIts; it++) held[it] = times(held[it], up);
+        }
 #pragma unroll
         for (int it = 0; it < kIts; it++) {
             const int i = it * kAppendThreads + tid;
-            if (i >= i0 && i < i1) *word(i) = scale > 0.f ? q8_encode4<kElem>(over(held[it], scale, inv)) : 0u;
+            if (i >= i0 && i < i1) *word(i) = scale > 0.f ? q8_encode4<kElem>(over(held[it], by, inv)) : 0u;
         }
     } else {
-        for (int i = i0 + tid; i < i1; i += kAppendThreads) *word(i) = scale > 0.f ? q8_encode4<kElem>(over(fetch(i), scale, inv)) : 0u;
+        for (int i = i0 + tid; i < i1; i += kAppendThreads) *word(i) = scale > 0.f ? q8_encode4<kElem>(over(times(fetch(i), up), by, inv)) : 0u;
     }
     if (tid == 0) *scales = scale;
 }

@@ -44,3 +44,33 @@ def test_a_page_whose_pieces_pass_32_bits_is_refused(block_size, head_dim):
     assert got.name == "InvalidArgument" and "block_size" in text
     got, text = _refusal(capi.lib.granite_cuda_rope_paged_kv_cache_append_q8, *_append_args(block_size=(1 << 30) - 32769, head_dim=8))
     assert got.name == "NullPointer" and "compute object" in text  # nothing left to refuse but the missing object
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", [0, 1])
+@pytest.mark.parametrize("block_size,d", [(16, 128), (16, 64), (8, 40)])
+@pytest.mark.parametrize("magnitude", [2.0 ** -117, 2.0 ** -110, 2.0 ** -100, 2.0 ** -80, 2.0 ** 100, 2.0 ** 126])
+def test_append_of_tiny_and_huge_values_writes_the_defined_bytes(compute, cache_dtype, block_size, d, magnitude):
+    """round(x / scale) to the last bit at both ends of the range, halves of a step among the values (where the quotient's last bit decides):
+    scales down to the smallest normal number, and up to a 127th of the largest."""
+    rng = np.random.default_rng(d)
+    hkv, n, batch = 4, 40, 3
+    qmax = R.QMAX[cache_dtype]
+    positions = np.array([0, 5, 17], np.int32)
+    pages = -(-(n + 17) // block_size)
+    tables = np.arange(batch * pages, dtype=np.int32).reshape(batch, pages)
+    pools = [R.random_pool(rng, tables.size, block_size, hkv, d, cache_dtype) for _ in range(2)]
+    codes, scales = [p[0] for p in pools], [(p[1] * magnitude / qmax).astype(np.float32) for p in pools]
+    # every value a whole or half number of steps of a page's likely scale, give or take a unit in the last place
+    top = (rng.uniform(1, 1.9, (batch, n, hkv, 1)) * magnitude).astype(np.float32)
+    x = ((rng.integers(-2 * int(qmax), 2 * int(qmax) + 1, (batch, n, hkv, d)) / (2 * qmax)).astype(np.float32) * top).astype(np.float32)
+    x[..., 0] = top[..., 0]
+    x = np.nextafter(x, np.float32(0) + rng.integers(-1, 2, x.shape).astype(np.float32) * np.float32(3e38))
+    v = x[:, ::-1].copy()
+    cos, sin = np.ones((n + 20, d // 2), np.float32), np.zeros((n + 20, d // 2), np.float32)
+    got = _run_append(compute, None, x, v, cos, sin, codes, scales, tables, positions, block_size, cache_dtype)
+    assert got[3] is None
+    want_codes, want_scales = [c.copy() for c in codes], [s.copy() for s in scales]
+    _append_reference(_rotate32(x, np.float32(1), np.float32(0)), want_codes[0], want_scales[0], tables, positions, block_size, cache_dtype, n + 20)
+    _append_reference(v, want_codes[1], want_scales[1], tables, positions, block_size, cache_dtype, n + 20)
+    _check_append(got, (want_codes, want_scales))
