@@ -858,44 +858,44 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         for (int h = 0; h < 2; h++) {
                             if (tree_step && h == 1) continue;
                             uint32_t hi[16], lo[16];
-            if constexpr (kQ8) {
+                            if constexpr (kQ8) {
 #pragma unroll
-                            for (int pg = 0; pg < 4; pg++) {
-                                const float iv = page_iv[4 * h + pg];
-                                const uint64_t iv2 = f32x2(iv, iv);
+                                for (int pg = 0; pg < 4; pg++) {
+                                    const float iv = page_iv[4 * h + pg];
+                                    const uint64_t iv2 = f32x2(iv, iv);
 #pragma unroll
-                                for (int q = 0; q < 2; q++) {
-                                    const float k = kSplitQ ? page_k[4 * h + pg] * q_step[q] : page_k[4 * h + pg];
-                                    const uint64_t k2 = f32x2(k, k);
-                                    // 2^(s k - m + log2(v / v_max)); masked scores are -inf and give exactly 0
-                                    const float off = page_lv[4 * h + pg] - m_used[q];
-                                    const uint64_t off2 = f32x2(off, off);
-                                    uint64_t pair[2];
+                                    for (int q = 0; q < 2; q++) {
+                                        const float k = kSplitQ ? page_k[4 * h + pg] * q_step[q] : page_k[4 * h + pg];
+                                        const uint64_t k2 = f32x2(k, k);
+                                        // 2^(s k - m + log2(v / v_max)); masked scores are -inf and give exactly 0
+                                        const float off = page_lv[4 * h + pg] - m_used[q];
+                                        const uint64_t off2 = f32x2(off, off);
+                                        uint64_t pair[2];
 #pragma unroll
-                                    for (int i2 = 0; i2 < 2; i2++) {
-                                        const int i = 2 * pg + i2;
-                                        float t0, t1;
-                                        f32x2_get(fma_f32x2(f32x2(__uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1])), k2, off2), t0, t1);
-                                        pair[i2] = f32x2(fast_exp2(t0), fast_exp2(t1));
-                                        split_hi_lo_x2(pair[i2], hi[2 * i + q], lo[2 * i + q]);
+                                        for (int i2 = 0; i2 < 2; i2++) {
+                                            const int i = 2 * pg + i2;
+                                            float t0, t1;
+                                            f32x2_get(fma_f32x2(f32x2(__uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1])), k2, off2), t0, t1);
+                                            pair[i2] = f32x2(fast_exp2(t0), fast_exp2(t1));
+                                            split_hi_lo_x2(pair[i2], hi[2 * i + q], lo[2 * i + q]);
+                                        }
+                                        ls[q][pg & 1] = fma_f32x2(add_f32x2(pair[0], pair[1]), iv2, ls[q][pg & 1]);
                                     }
-                                    ls[q][pg & 1] = fma_f32x2(add_f32x2(pair[0], pair[1]), iv2, ls[q][pg & 1]);
                                 }
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 8; i++)
+#pragma unroll
+                                    for (int q = 0; q < 2; q++) {
+                                        // masked scores are -inf: exp2 gives exactly 0
+                                        float t0, t1;
+                                        f32x2_get(fma_f32x2(f32x2(__uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1])),
+                                                            scale2, neg_m2[q]), t0, t1);
+                                        const uint64_t pp = f32x2(fast_exp2(t0), fast_exp2(t1));
+                                        ls[q][i & 1] = add_f32x2(ls[q][i & 1], pp);
+                                        split_hi_lo_x2(pp, hi[2 * i + q], lo[2 * i + q]);
+                                    }
                             }
-            } else {
-#pragma unroll
-                            for (int i = 0; i < 8; i++)
-#pragma unroll
-                                for (int q = 0; q < 2; q++) {
-                                    // masked scores are -inf: exp2 gives exactly 0
-                                    float t0, t1;
-                                    f32x2_get(fma_f32x2(f32x2(__uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1])),
-                                                        scale2, neg_m2[q]), t0, t1);
-                                    const uint64_t pp = f32x2(fast_exp2(t0), fast_exp2(t1));
-                                    ls[q][i & 1] = add_f32x2(ls[q][i & 1], pp);
-                                    split_hi_lo_x2(pp, hi[2 * i + q], lo[2 * i + q]);
-                                }
-            }
                             tmem_st_16x128b_x8(s_frag + 32 * h, hi);
                             tmem_st_16x128b_x8(s_frag + 64 + 32 * h, lo);
                         }

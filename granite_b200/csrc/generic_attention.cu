@@ -183,15 +183,16 @@ __global__ void __launch_bounds__(kGenThreads) generic_attention_kernel(GenericP
                     dot = fmaf(s_q[i + 7], b4.w, dot);
                 }
                 dot *= k_scale;
-            } else
-            for (int i = 0; i < p.d; i += 8) {  // head_dim is a multiple of 8: 16-byte pieces
-                const uint4 pk = *reinterpret_cast<const uint4*>(krow + i);
-                const __half2* h2 = reinterpret_cast<const __half2*>(&pk);
+            } else {
+                for (int i = 0; i < p.d; i += 8) {  // head_dim is a multiple of 8: 16-byte pieces
+                    const uint4 pk = *reinterpret_cast<const uint4*>(krow + i);
+                    const __half2* h2 = reinterpret_cast<const __half2*>(&pk);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float2 kf = __half22float2(h2[e]);
-                    dot = fmaf(s_q[i + 2 * e], kf.x, dot);
-                    dot = fmaf(s_q[i + 2 * e + 1], kf.y, dot);
+                    for (int e = 0; e < 4; e++) {
+                        const float2 kf = __half22float2(h2[e]);
+                        dot = fmaf(s_q[i + 2 * e], kf.x, dot);
+                        dot = fmaf(s_q[i + 2 * e + 1], kf.y, dot);
+                    }
                 }
             }
             s = dot * p.scale;

@@ -506,8 +506,8 @@ __device__ __forceinline__ void merge_direct(const DecodeParams& p, int b, int h
 #ifndef GB_DECODE_PAGES_PER_ITER_D64
 #define GB_DECODE_PAGES_PER_ITER_D64 2
 #endif
-// Pages that share one softmax round.  8-bit: one (two: 399 us against 370 for 64 sequences of up to 32768 tokens in e4m3 - the
-// registers for the second page's scores cost more than the shared round saves).
+// Pages that share one softmax round.  The 8-bit loop is written for one (a form of it with two took 399 us against 370 for 64 sequences
+// of up to 32768 tokens in e4m3 at head_dim 128, where registers are short: nine warps leave 168 a thread; at 64 it was not tried).
 __host__ __device__ constexpr int pages_per_iteration(int d, int elem) {
     return elem != kElemF16 ? 1 : d == 64 ? GB_DECODE_PAGES_PER_ITER_D64 : GB_DECODE_PAGES_PER_ITER_D128;
 }
@@ -596,7 +596,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
     constexpr int kHeadPageBytes = kPageTokens * D * (kElem == kElemF16 ? 2 : 1);  // one head's K (or V) page
     constexpr int NT = kTiles == 0 ? 1 : kTiles;
     constexpr bool kPair = kTiles == 0;
-    constexpr bool kMask = kWindow;  // rows of a page are masked by bit instead of by count
     extern __shared__ uint8_t smem_raw[];
     // 128-byte swizzle wants 1024-byte aligned slots
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -1132,7 +1131,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
             int ntok[PP], slot_k[PP], slot_v[PP];
             uint32_t ph_k[PP], ph_v[PP];
             bool has[PP];
-            uint32_t rows[PP];         // kMask: visible rows of the page
+            uint32_t rows[PP];         // kWindow: visible rows of the page, by bit (else they are counted: ntok)
 #pragma unroll
             for (int pp = 0; pp < PP; pp++) {
                 has[pp] = pp < here && j + pp < seg.npages;
@@ -1141,9 +1140,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                 ph_k[pp] = ph_v[pp] = 0;
                 rows[pp] = 0;
                 if (has[pp]) {
-                    if constexpr (kMask) {
+                    if constexpr (kWindow) {
                         const int v = seg.page_begin + j + pp;
-                        rows[pp] = page_rows<kWindow>(list, kWindow ? list.logical(v) : v, len);
+                        rows[pp] = page_rows<kWindow>(list, list.logical(v), len);
                     } else {
                         ntok[pp] = min(kPageTokens, len - (seg.page_begin + j + pp) * kPageTokens);
                     }
@@ -1185,7 +1184,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                     }
                 }
             }
-            if (kMask) fence_proxy_async_smem();  // the reads come before the next copy into the slot
+            if (kWindow) fence_proxy_async_smem();  // the reads come before the next copy into the slot
             __syncwarp();
             if (lane == 0) {
 #pragma unroll
@@ -1206,7 +1205,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                     s[pp][1] = sa[pp][nt][1] + sb_lo[pp][nt][1];
                     s[pp][2] = sa[pp][nt][2] + sb_lo[pp][nt][2];
                     s[pp][3] = sa[pp][nt][3] + sb_lo[pp][nt][3];
-                    if constexpr (kMask) {
+                    if constexpr (kWindow) {
                         if (!((rows[pp] >> g) & 1u)) s[pp][0] = s[pp][1] = -INFINITY;
                         if (!((rows[pp] >> (g + 8)) & 1u)) s[pp][2] = s[pp][3] = -INFINITY;
                     } else {
@@ -1252,7 +1251,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                 l_run[nt][1] = l_run[nt][1] * alpha1 + sum1;
                 alpha[nt][0] = alpha0;
                 alpha[nt][1] = alpha1;
-                if constexpr (!kMask) {
+                if constexpr (!kWindow) {
 #pragma unroll
                     for (int mt = 0; mt < kDSteps; mt++) {
                         o[nt][mt][0] *= alpha0;
@@ -1273,14 +1272,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                     if (lane == 0) atomicOr(p.status, kStatusTimeout);
                     return;
                 }
-                if (kMask ? rows[pp] != 0xFFFFu : ntok[pp] < kPageTokens) {
+                if (kWindow ? rows[pp] != 0xFFFFu : ntok[pp] < kPageTokens) {
                     // rows past the sequence end may hold anything (even NaN): zero them so that
                     // 0 * garbage cannot poison the accumulators
                     uint8_t* vptr = smem + (size_t)slot_v[pp] * slot_bytes + kvh_local * kHeadPageBytes;
                     constexpr int kRowUnits = D / 8;  // 16-byte units per row
-                    for (int i = lane; i < (kMask ? kPageTokens : kPageTokens - ntok[pp]) * kRowUnits; i += 32) {
-                        int r = (kMask ? 0 : ntok[pp]) + i / kRowUnits, u = i % kRowUnits;
-                        if (kMask && ((rows[pp] >> r) & 1u)) continue;
+                    for (int i = lane; i < (kWindow ? kPageTokens : kPageTokens - ntok[pp]) * kRowUnits; i += 32) {
+                        int r = (kWindow ? 0 : ntok[pp]) + i / kRowUnits, u = i % kRowUnits;
+                        if (kWindow && ((rows[pp] >> r) & 1u)) continue;
                         int chunk = u >> 3, unit = u & 7;
                         *reinterpret_cast<uint4*>(vptr + chunk * 2048 + r * 128 + ((unit ^ (r & 7)) << 4)) =
                             make_uint4(0, 0, 0, 0);
@@ -1308,15 +1307,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap kmap,
                     ldmatrix_x4_trans(a, vbase[pp] + (mt >> 2) * 2048 + ((unit ^ (v_row & 7)) << 4));
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        mma_16816(kMask ? acc[nt] : o[nt][mt], a, phi[pp][nt][0], phi[pp][nt][1]);
-                        mma_16816(kMask ? acc[nt] : o[nt][mt], a, plo[pp][nt][0], plo[pp][nt][1]);
+                        mma_16816(kWindow ? acc[nt] : o[nt][mt], a, phi[pp][nt][0], phi[pp][nt][1]);
+                        mma_16816(kWindow ? acc[nt] : o[nt][mt], a, plo[pp][nt][0], plo[pp][nt][1]);
                     }
                 }
-                if constexpr (kMask) fold(mt, acc);
+                if constexpr (kWindow) fold(mt, acc);
             }
             // Every lane's reads of the slots, and its zeros in rows that are not seen, come before the next copies into them: the fence is
             // each lane's own and stands before the barrier that lane 0 arrives behind.
-            bool written = kMask;
+            bool written = kWindow;
 #pragma unroll
             for (int pp = 0; pp < PP; pp++) written |= has[pp] && ntok[pp] < kPageTokens;
             if (written) fence_proxy_async_smem();
@@ -1737,7 +1736,7 @@ int launch_decode_as(granite_cuda_compute* c, const GraniteCudaPagedDecodeArgs& 
                         (int)a.batch_size * hkv <= kMaxDirectPairs;
     DecodeParams p{};
     size_t smem_bytes = 0;
-        if (!plan_decode_tile(p, direct ? 1 : tile_heads, group, D, c->smem_optin, &smem_bytes, kElem)) return plain();
+    if (!plan_decode_tile(p, direct ? 1 : tile_heads, group, D, c->smem_optin, &smem_bytes, kElem)) return plain();
     const int nt = p.heads_per_warp <= 8 ? 1 : 2;
     if (contiguous) {
         if (max_seq == 0) return fail(GRANITE_CUDA_INVALID_ARGUMENT, "decode: max_seq must be positive");
