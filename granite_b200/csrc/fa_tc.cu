@@ -37,10 +37,14 @@
 //               a finished item is read out behind the next item's first MMAs.
 // TMEM (512 columns): S[0] | S[1] | O[0] | O[1], 128 fp32 columns each.
 //
-// Two views of the cache have builds of their own (prefill only).  Their items may also be cut along the keys (n_chunks):
-// each chunk leaves its un-normalised output, maximum and sum per row, and prefill_merge_kernel joins them.  That fills the SMs
-// when there are few query blocks, and it bounds the number of truncating additions in a tensor-core accumulator: one run
-// over 6144 keys was off by 1.2e-5 (growing with the length), 18 tiles by 5.4e-6.
+// Two views of the cache have builds of their own (prefill only).  In them the hi and the lo products have an accumulator each (O[0] and
+// O[1]), which are added when an item is read out: with both issuers on one accumulator the order of their additions, and with
+// it the last bits of the result, changed from run to run, and the lo products truncated the sum as often as the hi ones
+// (5.4e-6 off over 18 tiles of fp32 queries, 2.9e-6 with two).  Nothing is left for the deferred read-out then: 41 us against 38 for
+// 2048 fp16 rows with a window of 512, no difference or a gain for longer items (2048 rows over 16384 keys: 654 us against 665).
+// Their items may also be cut along the keys (n_chunks): each chunk leaves its un-normalised output, maximum and sum per row, and
+// prefill_merge_kernel joins them.  That fills the SMs when there are few query blocks, and it bounds the number of
+// truncating additions in a tensor-core accumulator.
 //
 //   kWindow   sliding window with sinks.  A query block walks the tiles of the sinks and then those from the window of its first
 //             row to its diagonal, so its work is that of the keys it can see; tiles at the edges are masked by column.  Pages
@@ -245,6 +249,8 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
     static_assert(!(kSplitQ && kTiles == 2), "split queries take both query slots");
     using Item = std::conditional_t<kWindow, TcWindowItem, TcItem>;
     using Smem = TcSmem<Item>;
+    constexpr bool kTwoSums = kWindow;  // hi and lo products in accumulators of their own
+    static_assert(!kTwoSums || kTiles == 1, "both accumulators are taken");
     constexpr int kQSlots = kSplitQ ? 2 : kTiles;
     constexpr int kStages = kQSlots == 1 ? 3 : 2;
     // barriers first, then the 1024-byte aligned tiles (128-byte swizzle atoms)
@@ -565,7 +571,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     if (!it.valid) continue;
                     // one tile per item: O alternates between the two accumulators from item to item,
                     // so the previous item's result can be read out while this one accumulates
-                    const uint32_t o_sel = kTiles == 1 ? (items_done & 1) : 0;
+                    const uint32_t o_sel = kTwoSums ? part : kTiles == 1 ? (items_done & 1) : 0;
                     uint64_t* o_final = &sh->o_final[items_done & 1];
                     items_done++;
                     for (int j = 0; j < it.n_steps && ok; j++) {
@@ -622,7 +628,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
         // Read-out of a finished item.  With one tile per item it is deferred: the item's O stays in
         // its accumulator while the next item starts in the other one, and one 64-column half is
         // written after each of the next item's first softmax steps, behind the MMAs of those steps.
-        constexpr bool kDefer = kTiles == 1;
+        constexpr bool kDefer = kTiles == 1 && !kTwoSums;
         struct Readout {
             int halves_left;     // 0: nothing pending
             uint64_t* o_final;   // the item's "output MMAs done" barrier ...
@@ -647,6 +653,13 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
             __syncwarp();
             tmem_ld_16x256b_x8(e.o_frag + h * 64, rr);
             tmem_wait_ld();
+            if constexpr (kTwoSums) {
+                uint32_t lo[32];
+                tmem_ld_16x256b_x8(e.o_frag + kT + h * 64, lo);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; i++) rr[i] = __float_as_uint(__uint_as_float(rr[i]) + __uint_as_float(lo[i]));
+            }
             const bool partial = kWindow && p.n_chunks > 1;
             if (!kTree && p.out_fp16 && !partial) {
                 // a thread holds pairs of columns; a 4 x 4 exchange inside the quad turns four pairs of
@@ -721,7 +734,10 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                     }
 #pragma unroll
                     for (int h = 0; h < 2; h++)
-                        if (h < p.d_chunks) tmem_st_16x256b_x8(frag_base + 2 * kT + (t + o_sel) * kT + h * 64, z);  // own rows only
+                        if (h < p.d_chunks) {  // own rows only
+                            tmem_st_16x256b_x8(frag_base + 2 * kT + (t + o_sel) * kT + h * 64, z);
+                            if (kTwoSums) tmem_st_16x256b_x8(frag_base + 3 * kT + h * 64, z);
+                        }
                 }
                 tmem_wait_st();
             }
@@ -833,7 +849,8 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                             l_run[1] *= alpha1;
                             uint32_t rr[32];
 #pragma unroll 1
-                            for (int h = 0; h < p.d_chunks; h++) {
+                            for (int part = 0; part < (kTwoSums ? 2 : 1) * p.d_chunks; part++) {
+                                const int h = part < p.d_chunks ? part : part - p.d_chunks + 2;  // (64 columns; the lo sum is 128 further)
                                 tmem_ld_16x256b_x8(o_frag + h * 64, rr);
                                 tmem_wait_ld();
 #pragma unroll

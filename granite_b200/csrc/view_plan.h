@@ -54,8 +54,9 @@ GB_HOST_DEVICE WindowSteps window_steps(const PrefillSpan& p, int q0) {
 GB_HOST_DEVICE int chunk_begin(int n, int n_chunks, int c) { return n * c / n_chunks; }
 
 // ---- how a prefill's key tiles are cut into chunks (host)
-// A chunk's tiles run through one truncating tensor-core accumulator, 2.4e-9 of the result per key.  An fp32 output wants no more than
-// 22 of them (6.8e-6); an fp16 one 128, a twelfth of its own half step.
+// A chunk's tiles run through one truncating tensor-core accumulator, 1.3e-9 of the result per key.  An fp32 output wants no more than
+// 22 of them (3.6e-6): with 8, 4001 rows at 4099 under a window of 2047 are 1.4e-6 off instead of 2.9e-6 and take 369 us instead of
+// 275, with 4 1.0e-6 and 462 us.  An fp16 output wants no more than 128, a twentieth of its own half step.
 constexpr int kMaxChunks = 32;                       // the merge has one lane per chunk
 constexpr int kMaxTilesF32 = 22, kMaxTilesF16 = 128;
 constexpr size_t kMaxPartialBytes = (size_t)1 << 30;  // of a launch's partials: scratch that the object keeps
