@@ -489,18 +489,23 @@ typedef struct {
  * infinite K or V value does not enter the maximum, is stored as 0 and reported by granite_cuda_sync as
  * InvalidArgument.  A page that this call writes must belong to one sequence only (pages shared by several sequences
  * may be read by any number of them); a token that cannot be placed is skipped and reported as by the fp16 call.
- * head_dim: a multiple of 8, at most 256; any block_size. */
+ * head_dim: a multiple of 8, at most 256; any block_size up to a page of about 2^33 values per head. */
 int granite_cuda_rope_paged_kv_cache_append_q8(granite_cuda_compute_t* c, const GraniteCudaRopeAppendArgs* args,
                                                const GraniteCudaQ8Cache* cache);
 
 /* granite_cuda_batched_paged_attention_decode over the 8-bit cache; window may be NULL.  Tuned kernel: head_dim 128
  * or 64, block_size 16; other head dims (multiples of 8 up to 256) and page sizes run on a plain fp32 kernel.  Codes
- * and scales are not rounded on the way: results have the accuracy of fp32 arithmetic on the values held. */
+ * and scales are not rounded on the way: results have the accuracy of fp32 arithmetic on the values held, whatever the
+ * magnitudes of queries and page scales.  Q itself is taken to 24 bits of a head's largest element (int8), or to 22 bits of
+ * every element that is at least 2^-14 of it (e4m3).  The same call gives the same bits every time. */
 int granite_cuda_batched_paged_attention_decode_q8(granite_cuda_compute_t* c, const GraniteCudaPagedDecodeArgs* args,
                                                    const GraniteCudaQ8Cache* cache, const GraniteCudaAttentionWindow* window);
 
 /* granite_cuda_paged_prefill_attention over the 8-bit cache; window may be NULL.  Same shapes as the fp16 call.  The visible
- * codes are laid out as fp16 in the object's scratch first (4 bytes per key, KV head and dim), and the keys may be cut into
+ * codes are laid out as fp16 in the object's scratch first (4 bytes per key, KV head and dim).  Accuracy as for decode (fp32 Q
+ * like e4m3's there), but for the sums: a tensor-core accumulator truncates, by about 1.3e-9 of the result per key that runs through
+ * it, 2816 keys at most for fp32 outputs and 16384 for fp16 ones (a 32nd of the keys beyond 90112 and 524288); V scales
+ * below 2^-100 of the largest that the call sees count as that.  The same call gives the same bits every time.  The keys may be cut into
  * chunks whose partial results, up to 1 GiB of them, are kept there too; a call that would need more runs as several
  * launches over some of its rows each. */
 int granite_cuda_paged_prefill_attention_q8(granite_cuda_compute_t* c, const GraniteCudaPagedPrefillArgs* args,
@@ -510,7 +515,8 @@ int granite_cuda_paged_prefill_attention_q8(granite_cuda_compute_t* c, const Gra
  * The three calls without the suffix, restricted to the keys that the window leaves visible.  A sequence's query
  * positions are those of the plain calls (decode: the last token; prefill: start_pos + i).  Pages that no query of the
  * call sees are not read and their table entries are not looked at, so a host may free them.  A query row that sees no
- * key at all (contiguous prefill with seq_kv short of the window's start) gets zeros.  Prefill keeps partial results of keys
+ * key at all (contiguous prefill with seq_kv short of the window's start) gets zeros.  The same call gives the same bits every
+ * time; sums as described for the 8-bit prefill above.  Prefill keeps partial results of keys
  * that are cut into chunks in the object's scratch, up to 1 GiB (see above). */
 int granite_cuda_batched_paged_attention_decode_window(granite_cuda_compute_t* c, const GraniteCudaPagedDecodeArgs* args,
                                                        const GraniteCudaAttentionWindow* window);
