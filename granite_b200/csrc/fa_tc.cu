@@ -76,6 +76,7 @@ constexpr int kPageRows = 16;
 constexpr float kLazyLog2 = 8.0f;
 constexpr int kMaxStages = 3;
 constexpr uint32_t kNegInf = 0xFF800000u;
+constexpr float kSmallestNormal = 0x1p-126f;
 
 struct TcParams {
     int num_heads, num_kv_heads, group;
@@ -761,6 +762,10 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                         page_lv[4 * c] = b.x; page_lv[4 * c + 1] = b.y; page_lv[4 * c + 2] = b.z; page_lv[4 * c + 3] = b.w;
                     }
                 }
+                // what a score of page pg and row q is multiplied by: a positive number in any case, since masked scores are -infinity
+                // (a row of zeros has the smallest step, a page of zeros the smallest scale: below the normal numbers the product
+                // of a score that is not masked is next to nothing)
+                auto k_factor = [&](int pg, int q) { return kSplitQ ? fmaxf(page_k[pg] * q_step[q], kSmallestNormal) : page_k[pg]; };
                 // not unrolled: the two tiles of an item share one copy of the softmax code
 #pragma unroll 1
                 for (int t = 0; t < kTiles; t++, vs++) {
@@ -821,7 +826,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                                     const float pm = fmaxf(max3(__uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1]),
                                                                 __uint_as_float(x[h][4 * i + 4 + 2 * q])),
                                                            __uint_as_float(x[h][4 * i + 4 + 2 * q + 1]));
-                                    mm[h] = fmaxf(mm[h], fmaf(pm, kSplitQ ? page_k[4 * h + i / 2] * q_step[q] : page_k[4 * h + i / 2], page_lv[4 * h + i / 2]));
+                                    mm[h] = fmaxf(mm[h], fmaf(pm, k_factor(4 * h + i / 2, q), page_lv[4 * h + i / 2]));
                                 } else {
                                     mm[h] = max3(mm[h], __uint_as_float(x[h][4 * i + 2 * q]), __uint_as_float(x[h][4 * i + 2 * q + 1]));
                                 }
@@ -882,7 +887,7 @@ fa_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ C
                                     const uint64_t iv2 = f32x2(iv, iv);
 #pragma unroll
                                     for (int q = 0; q < 2; q++) {
-                                        const float k = kSplitQ ? page_k[4 * h + pg] * q_step[q] : page_k[4 * h + pg];
+                                        const float k = k_factor(4 * h + pg, q);
                                         const uint64_t k2 = f32x2(k, k);
                                         // 2^(s k - m + log2(v / v_max)); masked scores are -inf and give exactly 0
                                         const float off = page_lv[4 * h + pg] - m_used[q];
@@ -1359,14 +1364,13 @@ __global__ void __launch_bounds__(256) q8_gather_kernel(const __grid_constant__ 
                     v = p.v_scales[(size_t)e * p.hkv + h];
                 }
             }
-            // Scale 0 comes with zero codes, so any positive number stands for it.  V scales count as 2^-100 of the call's
+            // Scale 0 comes with zero codes, so any positive number stands for it (masked scores are -infinity).  V scales count as 2^-100 of the call's
             // largest at least: a page of tiny values may hold most of a row's weight, and that weight is counted through its
             // product 2^(s k scale - m) r.  m is at most the row's largest score, so the product of the page with that score is at
             // least 2^-100, a normal number, and no weight passes 2^108.
-            k = fmaxf(k, 1e-30f);
             const float r = fmaxf(__fdiv_rn(v, m), 7.88860905e-31f);
             const size_t at = (size_t)h * p.page_stride + page;
-            p.page_k[at] = k * p.scale_log2;
+            p.page_k[at] = fmaxf(k * p.scale_log2, kSmallestNormal);
             p.page_lv[at] = log2f(r);
             p.page_iv[at] = __fdiv_rn(1.f, r);
         }

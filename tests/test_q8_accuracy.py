@@ -160,7 +160,7 @@ def small_query_case(rng, n, rows, hq, hkv, d, cache_dtype, magnitude):
 @pytest.mark.gpu
 @pytest.mark.parametrize("cache_dtype", [0, 1])
 @pytest.mark.parametrize("hq,hkv,d,n", [(8, 2, 128, 700), (32, 4, 64, 100), (16, 1, 128, 1500)])
-@pytest.mark.parametrize("magnitude", [1e-2, 1e-4, 1e-9, 1e-20, 1e6])
+@pytest.mark.parametrize("magnitude", [1e-2, 1e-4, 1e-9, 1e-20, 1e-30, 1e6, 1e30])
 def test_decode_q8_queries_of_any_magnitude(compute, cache_dtype, hq, hkv, d, n, magnitude):
     """q . k is the same product whichever of the two holds the magnitude."""
     import torch
@@ -177,7 +177,7 @@ def test_decode_q8_queries_of_any_magnitude(compute, cache_dtype, hq, hkv, d, n,
 @pytest.mark.gpu
 @pytest.mark.parametrize("cache_dtype", [0, 1])
 @pytest.mark.parametrize("hq,hkv,d,seq,start", [(8, 2, 128, 130, 300), (32, 4, 64, 3, 60), (2, 1, 128, 257, 0)])
-@pytest.mark.parametrize("magnitude", [1e-2, 1e-4, 1e-9, 1e-20, 1e6])
+@pytest.mark.parametrize("magnitude", [1e-2, 1e-4, 1e-9, 1e-20, 1e-30, 1e6, 1e30])
 def test_prefill_q8_queries_of_any_magnitude(compute, cache_dtype, hq, hkv, d, seq, start, magnitude):
     import torch
     rng = np.random.default_rng(seq)
@@ -208,3 +208,35 @@ def test_prefill_q8_a_query_that_is_not_finite_spoils_its_own_row_and_head(compu
     for r, h in ((5, 1), (130, 2)):
         got[r, h] = want[r, h]
     check(got, want, bound, norm, "the other rows and heads")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache_dtype", [0, 1])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("d", [128, 64])
+@pytest.mark.parametrize("k_scale", [0.0, 1e-7, 1e-30, 2.0 ** -126])
+def test_prefill_q8_rows_of_zeros_meet_pages_of_zeros(compute, cache_dtype, half, d, k_scale):
+    """Query rows of zeros (padding), pages of zero or next to zero keys, in tiles whose later keys are masked: the factor that takes a masked
+    score to the base-2 exponent must not vanish.  A row of zeros is the mean of what it sees."""
+    import torch
+    rng = np.random.default_rng(d)
+    hq, hkv, seq, start = 4, 2, 150, 40
+    n = seq + start
+    t, blocks, q, kc, ks, vc, vs = small_query_case(rng, n, seq, hq, hkv, d, cache_dtype, 1.0)
+    kc, ks = kc.copy(), ks.copy()
+    q[3], q[64:70, 1], q[149] = 0, 0, 0
+    q[80] *= 1e-20 if not half else 0
+    if half:
+        q = q.astype(np.float16).astype(np.float32)
+    for p in (0, 4, 5, 9, 11):
+        e = t[0, p]
+        ks[e] = k_scale
+        if k_scale == 0:
+            kc[e * 16:e * 16 + 16] = 0
+    ref = weighted_reference(q.astype(np.float64), kc, ks, vc, vs, start + np.arange(seq), d ** -0.5, cache_dtype, t[0])
+    dt = torch.float16 if half else torch.float32
+    out = torch.full(q.shape, float("nan"), device=DEV)
+    compute.paged_prefill_attention_q8(_dev(q, dt), *[_dev(x) for x in (kc, vc, ks, vs, t)], out, hq, hkv, seq, start, d, 16, t.shape[1], blocks, d ** -0.5, cache_dtype,
+                                       q_dtype=int(half), out_dtype=0)
+    compute.sync()
+    check(out.cpu().numpy(), *ref, f"K scale {k_scale}")
