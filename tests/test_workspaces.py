@@ -205,3 +205,27 @@ def test_a_prefill_without_room_for_partials_runs_in_one_chunk():
     assert float((outs[0] - outs[1]).norm() / outs[0].norm()) <= 2.4e-9 * n
     roomy.shutdown()
     tight.shutdown()
+
+
+@pytest.mark.gpu
+def test_a_batch_of_long_prefills_runs_sequence_by_sequence():
+    """The partials of the batch pass the limit, those of one sequence do not: the same rows as three calls give, in fp32 from fp16 queries."""
+    import torch
+    import granite_b200 as g
+    hq, hkv, d, seq, n, batch = 64, 1, 64, 1500, 98000, 3
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(4)
+    q = torch.empty((batch, seq, hq, d), device=DEV).normal_(generator=gen).half()
+    k, v = (torch.empty((batch, hkv, n, d), device=DEV).normal_(generator=gen).half() for _ in range(2))
+    outs = [torch.zeros((batch, seq, hq, d), device=DEV) for _ in range(2)]
+    o = g.CudaCompute(0)
+    torch.cuda.synchronize()
+    args = (hq, hkv, seq, n - 100, d, d ** -0.5, 97000, 4, n)
+    before = o.get_profiling_stats()[0]
+    o.multihead_attention_window(q, k, v, outs[0], *args, q_dtype=1, start_pos=n - 100 - seq, batch_size=batch)
+    assert o.get_profiling_stats()[0] - before == 2 * batch  # attention and merge of each
+    for b in range(batch):
+        o.multihead_attention_window(q[b], k[b], v[b], outs[1][b], *args, q_dtype=1, start_pos=n - 100 - seq)
+    o.sync()
+    assert torch.equal(outs[0], outs[1]) and bool(outs[0].any())
+    o.shutdown()
