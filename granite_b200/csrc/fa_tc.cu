@@ -1104,16 +1104,19 @@ static int ensure_with_partials(granite_cuda_compute* c, TcParams& p, size_t fix
     }
     return rc;
 }
-// A call whose partials pass the limit runs as several, each on some of the query rows.
+// A call whose partials pass the limit runs as several, each on some of the query rows: the last rows first, since they need the most
+// scratch (the arena grows once, and a call that may not grow it is refused before anything of it runs).
 template <typename Args, typename Launch>
 static int launch_by_rows(const Args& a, uint32_t rows, Launch launch) {
     const size_t elements = (size_t)a.num_heads * a.head_dim;
-    for (uint32_t s0 = 0; s0 < a.seq_q; s0 += rows) {
+    for (uint32_t left = a.seq_q; left > 0;) {
+        const uint32_t n = std::min(rows, left), s0 = left - n;
+        left = s0;
         Args part = a;
         part.q = static_cast<const char*>(a.q) + s0 * elements * (a.q_dtype == 0 ? 4 : 2);
         part.output = static_cast<char*>(a.output) + s0 * elements * (a.out_dtype == 0 ? 4 : 2);
         part.start_pos = a.start_pos + s0;
-        part.seq_q = std::min(rows, a.seq_q - s0);
+        part.seq_q = n;
         if (int rc = launch(part)) return rc;
     }
     return GRANITE_CUDA_SUCCESS;

@@ -162,7 +162,7 @@ def test_a_prefill_of_many_rows_over_a_long_context_runs_in_several_launches(kin
     # partials of 1 GiB, the queries' halves, the 8-bit cache's fp16 copy, a quarter more
     assert free - torch.cuda.mem_get_info(0)[0] <= 1.25 * ((1 << 30) + q.numel() * 4 + 4 * n * d + (1 << 20)) + (64 << 20)
     k, v = (x[0].double() for x in kv)
-    for rows in (slice(0, 3), slice(1916, 1926), slice(seq - 3, seq)):
+    for rows in (slice(0, 3), slice(seq - 2 * 1920 - 5, seq - 2 * 1920 + 5), slice(seq - 1925, seq - 1915), slice(seq - 3, seq)):
         pos = start + torch.arange(seq, device=DEV)[rows]
         j = torch.arange(n, device=DEV)
         seen = (j <= pos[:, None]) & ((pos[:, None] - j < window) | (j < sinks))
@@ -205,6 +205,55 @@ def test_a_prefill_without_room_for_partials_runs_in_one_chunk():
     assert float((outs[0] - outs[1]).norm() / outs[0].norm()) <= 2.4e-9 * n
     roomy.shutdown()
     tight.shutdown()
+
+
+@pytest.mark.gpu
+def test_a_prefill_of_several_launches_is_captured_whole_or_not_at_all():
+    """Every launch of it needs scratch of its own size, the one over the last rows the most: where the arena cannot grow, nothing is captured of
+    the call."""
+    import torch
+    import granite_b200 as g
+    hq, hkv, d, seq, start = 64, 1, 64, 2500, 96000
+    n = seq + start
+    blocks = (n + 15) // 16
+    side = torch.cuda.Stream(device=DEV)
+    o = g.CudaCompute(0, side.cuda_stream)
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(5)
+    q = torch.empty((seq, hq, d), device=DEV).normal_(generator=gen)
+    k, v = (torch.randint(-127, 128, (blocks * 16, hkv, d), device=DEV, generator=gen, dtype=torch.int8) for _ in range(2))
+    scales = torch.full((blocks, hkv), 1 / 40, device=DEV)
+    table = torch.arange(blocks, device=DEV, dtype=torch.int32)
+    outs = [torch.zeros_like(q) for _ in range(2)]
+
+    def call(out, rows, first):
+        o.paged_prefill_attention_q8(q[first:first + rows], k, v, scales, scales, table, out[first:first + rows], hq, hkv, rows, start + first, d, 16, blocks, blocks,
+                                     d ** -0.5, 0)
+
+    torch.cuda.synchronize()
+    call(outs[0], 1000, 0)  # half of what the call's launches need
+    o.sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="relaxed"):
+        before = o.get_profiling_stats()[0]
+        with pytest.raises(g.GraniteCudaError) as e:
+            call(outs[1], seq, 0)
+        assert e.value.code == g.ErrorCode.InvalidState and o.get_profiling_stats()[0] == before
+    call(outs[1], seq, 0)  # two launches, over rows 580 to 2499 and 0 to 579
+    o.sync()
+    outs[1].zero_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="relaxed"):
+        call(outs[1], seq, 0)
+    graph.replay()
+    torch.cuda.synchronize()
+    call(outs[0], 1500, 1000)
+    o.sync()
+    # (the two are cut elsewhere along the rows and keys: equal to the error of their sums)
+    assert float((outs[0] - outs[1]).norm() / outs[0].norm()) < 1e-5
+    del graph
+    o.shutdown()
 
 
 @pytest.mark.gpu
